@@ -98,11 +98,11 @@ def prepare(case, seed):
         s["Wg"], s["Wu"] = rnd(D, F) / math.sqrt(D), rnd(D, F) / math.sqrt(D)
         s["Wd"] = rnd(F, D) / math.sqrt(F)
         s["H"], s["Y"] = buf(N, F), buf(N, D)
+        s["work"] = buf(32 << 20)        # partial sums of split products, kept by the program
         if case["train"]:
             s["dY"] = rnd(N, D) * 1e-2
             s["G"], s["U"], s["dG"], s["dU"] = buf(N, F), buf(N, F), buf(N, F), buf(N, F)
             s["dX"], s["dWg"], s["dWu"], s["dWd"] = buf(N, D), buf(D, F), buf(D, F), buf(F, D)
-            s["work"] = buf(32 << 20)    # partial sums of the weight gradients, kept by the program
         return s
     if case["op"] == "norm":
         N, M, P = case["N"], case["M"], _pad4(case["M"])
@@ -252,7 +252,7 @@ def _own(s):
     if s["op"] == "ff":
         ff, act = cu32.Cuda_gatedFF, ACTS.index(s["act"])
         ff.gatedFF([stream], 1, p("X"), p("Wg"), p("Wu"), p("Wd"), p("G"), p("U"), p("H"), p("Y"),
-                   s["N"], s["D"], s["F"], act)
+                   p("work"), s["work"].numel(), s["N"], s["D"], s["F"], act)
         if not s["train"]:
             return [s["Y"]]
         ff.gatedFF_delta([stream], 1, p("dY"), p("X"), p("Wg"), p("Wu"), p("Wd"), p("G"), p("U"), p("H"),
