@@ -15,7 +15,7 @@
 #include <mutex>
 
 #include "../../include/dragon_cu32.h"
-#include "gemm_launch.h"
+#include "cu32_host.h"
 
 namespace dragon {
 
@@ -36,7 +36,7 @@ static std::atomic<int> g_ring_paired{1};
 static std::atomic<int> g_ring_fixed{1};
 static std::atomic<int> g_phase_fused{1};
 
-static void load_env_once() {
+void load_env_once() {
   static std::once_flag once;
   std::call_once(once, [] {
     if (const char* s = std::getenv("DRAGON_CU32_KC")) { int v = std::atoi(s); if (v >= 1) g_kc = v; }
@@ -52,7 +52,7 @@ static void load_env_once() {
 // ------------------------------------------------------------------ device status word
 __device__ int g_status_word;
 
-static int* status_word_ptr(cudaError_t* err) {
+int* status_word_ptr(cudaError_t* err) {
   // The symbol has one instance per device; cache its address per device ordinal.
   static std::atomic<int*> cache[64];
   int dev = 0;
@@ -98,7 +98,7 @@ typedef CUresult (*EncodeIm2colFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
 static EncodeTiledFn g_encode_tiled = nullptr;
 static EncodeIm2colFn g_encode_im2col = nullptr;
 
-static bool load_driver_entry_points() {
+bool load_driver_entry_points() {
   static std::once_flag once;
   std::call_once(once, [] {
     void* fn = nullptr;
@@ -118,7 +118,7 @@ static bool load_driver_entry_points() {
 // (reduction axis innermost) use the plain 128-byte swizzle; MN-major operands use the
 // 128-byte swizzle with 32-byte units, the only one the tensor core reads for 32-bit
 // MN-major tiles.
-static int make_map3(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint64_t d2,
+int make_map3(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint64_t d2,
                      uint64_t pitch1_floats, uint64_t pitch2_floats, uint32_t b0, uint32_t b1,
                      bool mn_major) {
   cuuint64_t dims[3] = {d0, d1, d2};
@@ -131,27 +131,6 @@ static int make_map3(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? CU32_OK : CU32_E_TENSORMAP;
 }
-
-// One contraction, BLAS letters: C[M,N] = A * B over K.
-struct GemmCall {
-  const float* A; const float* B; float* C; float* Cbuf;
-  int M, N, K;              // logical extents of the operands
-  int n_store;              // columns of C written (>= N; columns N.. come out 0)
-  long long lda, ldb, ldc;  // row pitches in floats
-  bool a_mn, b_mn;          // operand stored with its M / N axis contiguous
-  int batch; long long sA, sB, sC;
-  int gz;                   // split-K slices (1 = none)
-  bool x3;                  // FP32-accurate (true) or single-pass TF32
-  cudaStream_t stream;
-  const float* bias;        // optional row vector (n_store floats) added in the epilogue; needs gz == 1, batch == 1
-  int bias_width;           // true width of the rows: columns beyond it are stored as zeros
-  bool scale_on = false;   // store alpha * result (one rounding), vector store paths only
-  float alpha = 1.0f;
-  float* const* replicas = nullptr;   // further output buffers that receive the same stores as C (same layout)
-  int n_replicas = 0;
-};
-
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Tile choice: estimated time = waves over the SMs x work per CTA / measured per-CTA
 // rate.  The rates are FP32-accurate TFLOP/s measured at 8192^3 on a B200 with every SM
@@ -173,7 +152,7 @@ static int pick_tile_auto(long long M, int N, long long z) {
   return best;
 }
 // The tile a call uses: the forced one if a tuning key set it, else the estimate's; remembered for diagnostics.
-static int note_tile(int t) { g_last_tile = t; return t; }
+int note_tile(int t) { g_last_tile = t; return t; }
 static int pick_tile(long long M, int N, long long z) {
   const int forced = g_tile.load();
   return note_tile(forced >= 0 ? forced : pick_tile_auto(M, N, z));
@@ -182,7 +161,9 @@ static int pick_tile(long long M, int N, long long z) {
 // Ring lengths for a launch (see GemmParams): explicit tuning values win, otherwise 0 = the kernel
 // configuration's balanced default.
 // Also sets how many chunks are summed in registers between flushes to memory: 256 k-blocks (K = 8192).
-static void choose_rings(GemmParams* p) {
+int tuned_kc() { return g_kc.load(); }
+int forced_tile() { return g_tile.load(); }
+void choose_rings(GemmParams* p) {
   p->flush_chunks = 256 / p->kc > 1 ? 256 / p->kc : 1;
   p->ring_raw = g_ring_raw.load();
   p->ring_lo = g_ring_lo.load();
@@ -196,7 +177,7 @@ static void choose_rings(GemmParams* p) {
   p->clock_acc = clock_acc_ptr();
 }
 
-static int run_gemm(const GemmCall& c) {
+int run_gemm(const GemmCall& c) {
   load_env_once();
   if (!c.A || !c.B || !c.C) return CU32_E_NULL;
   if (c.gz > 1 && !c.Cbuf) return CU32_E_NULL;
@@ -300,7 +281,7 @@ static int run_gemm(const GemmCall& c) {
   return static_cast<int>(e);
 }
 
-static int check_streams(const int64_t* streams, int length, cudaStream_t* s0) {
+int check_streams(const int64_t* streams, int length, cudaStream_t* s0) {
   if (!streams || length < 1 || length > 10) return CU32_E_STREAMS;
   *s0 = reinterpret_cast<cudaStream_t>(static_cast<intptr_t>(streams[0]));
   return CU32_OK;

@@ -41,6 +41,7 @@
 // records (role, stage, iteration) in the status word, raises the CTA's abort
 // flag, and all roles fall through to the common exit, which frees TMEM.
 #pragma once
+#include "gated_act.cuh"
 #include "sm100_ptx.cuh"
 
 namespace dragon {
@@ -69,6 +70,8 @@ struct GemmParams {
   CUtensorMap tmCbuf;   // split-K partial buffers: dims (N, M, gz-1), same box
   CUtensorMap tmRep[7];  // further copies of the output (same dims and box as tmC), e.g. the same rows of a gathered
                          // output in the memory of the other GPUs of an NVLink domain, mapped into this process
+                         // EPI_GATED: [0], [1] = the saved pre-activations G and U (maps like tmC), [3] = the second
+                         // weight (a map like tmB);  EPI_DUAL: [2], [3] = the second product's A and B
   int n_rep;             // how many of them are valid: every store to C is repeated to each (stores only, never loads)
   float* rep_ptr[7];     // the same copies as plain pointers (same pitch as C), for the lazy mode below
   int rep_lazy;          // 1: the drain warps store a finished block to C only and carry it to the copies while the
@@ -136,12 +139,27 @@ struct GemmParams {
   // phase's tile run under the MMAs of the next, longer one.  Phase 0 is described by the fields above.
   int n_phases;
   GemmPhase phx[3];
+  // Gated feed-forward block (the EPI_* instantiations)
+  int act;              // activation, CU32_ACT_*
+  int gated_save;       // EPI_GATED: store G and U too
+  int nkb_first;        // EPI_DUAL: k-blocks of the first product; the rest belong to the second
+  const float* ep_g;    // EPI_DGATED: G, U [M, N] read, deltaG, deltaU written, all with C's pitch (the outputs may
+  const float* ep_u;    // be the inputs' own buffers)
+  float* ep_dg;
+  float* ep_du;
 };
+
+// What happens to a finished tile beyond the plain store:
+//   EPI_GATED   the tile's columns are two interleaved products A*B and A*B2 of the same hidden units: act(G) * U is
+//               stored (and G and U, when asked), a tile covers BN / 2 hidden units
+//   EPI_DGATED  the tile is deltaH: deltaG = deltaH * U * act'(G) and deltaU = deltaH * act(G) are stored instead
+//   EPI_DUAL    C = A*B + A2*B2, the second product's k-blocks behind the first's
+enum GemmEpilogue : int { EPI_NONE = 0, EPI_GATED = 1, EPI_DGATED = 2, EPI_DUAL = 3 };
 
 enum GemmRole : int { ROLE_TMA = 1, ROLE_SPLIT = 2, ROLE_MMA = 3, ROLE_MMA_TMEM = 4, ROLE_DRAIN = 5, ROLE_SELFTEST = 7 };
 
 template <int BN_, int CTAS_, bool A_MN_, bool B_MN_, bool X3_, bool IM2COL_ = false, bool SOFTMAX_ = false,
-          bool REP_ = false>
+          bool REP_ = false, int EPI_ = EPI_NONE>
 struct GemmCfg {
   static constexpr int BN = BN_, CTAS = CTAS_;
   static constexpr bool A_MN = A_MN_, B_MN = B_MN_, X3 = X3_, IM2COL = IM2COL_;
@@ -151,6 +169,11 @@ struct GemmCfg {
   // REP: the output is kept in up to seven further copies (GemmParams::tmRep / rep_ptr); the other
   // instantiations carry none of that code.
   static constexpr bool REP = REP_;
+  static constexpr int EPI = EPI_;
+  static_assert(EPI_ != EPI_GATED || (!A_MN_ && B_MN_ && X3_ && !IM2COL_ && BN_ >= 128), "gated: A[M][K] x B[K][N]");
+  static_assert((EPI_ != EPI_DGATED && EPI_ != EPI_DUAL) || (!A_MN_ && !B_MN_ && X3_ && !IM2COL_),
+                "gated gradients: A[M][K] x B[N][K]^T");
+  static constexpr int OUT_BN = EPI_ == EPI_GATED ? BN_ / 2 : BN_;   // output columns of a tile
   static_assert(!SOFTMAX_ || (BN_ == 256 && CTAS_ == 2 && X3_ && !A_MN_ && !B_MN_ && !IM2COL_),
                 "the row softmax is built on the 256x256 pair tile of the A * B^T form");
   static constexpr int BM = 128;            // rows of A (and TMEM lanes) per CTA
@@ -171,7 +194,7 @@ struct GemmCfg {
   // the below-ridge geometry (measured on the attention-shaped batched products): 128x64 one-CTA tile 6 raw + 2 lo
   // slots, 256x256 pair tile 3 + 2 with two staging tiles per drain warp (3 + 2 + 1 with the fused softmax, which
   // needs the room for its row statistics); 0 = the configuration has none
-  static constexpr bool ALT_OK = X3 && !IM2COL_ && ((BN == 64 && CTAS == 1) || (BN == 256 && CTAS == 2));
+  static constexpr bool ALT_OK = X3 && !IM2COL_ && EPI_ == EPI_NONE && ((BN == 64 && CTAS == 1) || (BN == 256 && CTAS == 2));
   static constexpr int ALT_RAW = !ALT_OK ? 0 : (BN == 64 ? 6 : 3);
   static constexpr int ALT_LO = !ALT_OK ? 0 : 2;
   static constexpr int ALT_BUFS = !ALT_OK ? 0 : (BN == 64 || SOFTMAX_ ? 1 : 2);
@@ -344,7 +367,7 @@ __device__ __forceinline__ void gemm_tf32_body(const GemmParams& p) {
     const int tn = Cfg::SOFTMAX ? r % p.tiles_n : (r % per_group) / g_size;
     TileWork w;
     w.row0 = (tm * CTAS + static_cast<int>(rank)) * Cfg::BM;
-    w.col0 = tn * BN;
+    w.col0 = tn * Cfg::OUT_BN;
     w.bcol0 = w.col0 + static_cast<int>(rank) * Cfg::BN_CTA;
     w.tap = 0;
     w.phase = phase;
@@ -504,6 +527,8 @@ __device__ __forceinline__ void gemm_tf32_body(const GemmParams& p) {
             oh = r / p.conv_OW;
             ow = r - oh * p.conv_OW;
           }
+          const bool second = Cfg::EPI == EPI_DUAL && w.kb0 + i >= p.nkb_first;   // the second product's operands
+          if (second) k0 -= p.nkb_first * Cfg::BK;
           uint32_t tx_bytes = Cfg::HI_BYTES;
           if (Cfg::IM2COL && p.gather) {
             // Slow path: the whole warp builds the im2col tile with 16-byte loads, zero outside the image, in the
@@ -571,7 +596,7 @@ __device__ __forceinline__ void gemm_tf32_body(const GemmParams& p) {
               for (int j = 0; j < Cfg::BM / 32; ++j)
                 tma_load_3d(a_dst + j * 4096, &p.tmA, full, w.row0 + 32 * j, k0, w.batch, pol_a);
             } else {
-              tma_load_3d(a_dst, &p.tmA, full, k0, w.row0, w.batch, pol_a);
+              tma_load_3d(a_dst, second ? &p.tmRep[2] : &p.tmA, full, k0, w.row0, w.batch, pol_a);
             }
             if (Cfg::IM2COL_B && p.gather) {
               // the B slabs are in place already
@@ -592,12 +617,22 @@ __device__ __forceinline__ void gemm_tf32_body(const GemmParams& p) {
               for (int j = 0; j < Cfg::BN_CTA / 32; ++j)
                 if (p.bmap_order == 0) tma_load_3d(b_dst + j * 4096, pv.tmB, full, w.bcol0 + 32 * j, btap, ic0, pol_b);
                 else                   tma_load_3d(b_dst + j * 4096, pv.tmB, full, w.bcol0 + 32 * j, ic0, btap, pol_b);
+            } else if (Cfg::EPI == EPI_GATED) {
+              // The tile's columns: for each drain-warp half, CW / 2 columns of the first weight, then the same hidden
+              // units' columns of the second, so that one thread's accumulators hold G and U of the same elements.
+#pragma unroll
+              for (int j = 0; j < Cfg::BN_CTA / 32; ++j) {
+                const int jg = static_cast<int>(rank) * (Cfg::BN_CTA / 32) + j;
+                const int hh = jg / (CW / 32), wi = jg % (CW / 32);
+                tma_load_3d(b_dst + j * 4096, wi < CW / 64 ? &p.tmB : &p.tmRep[3], full,
+                            w.col0 + hh * (CW / 2) + (wi % (CW / 64)) * 32, k0, w.batch, pol_b);
+              }
             } else if (Cfg::B_MN) {
 #pragma unroll
               for (int j = 0; j < Cfg::BN_CTA / 32; ++j)
                 tma_load_3d(b_dst + j * 4096, &p.tmB, full, w.bcol0 + 32 * j, k0, w.batch, pol_b);
             } else {
-              tma_load_3d(b_dst, &p.tmB, full, k0, w.bcol0, w.batch, pol_b);
+              tma_load_3d(b_dst, second ? &p.tmRep[3] : &p.tmB, full, k0, w.bcol0, w.batch, pol_b);
             }
           }
           __syncwarp();
@@ -1081,7 +1116,92 @@ __device__ __forceinline__ void gemm_tf32_body(const GemmParams& p) {
           return v;
         };
         // ---- store; the MMA warp is already filling the TMEM buffers with the next chunks meanwhile
-        if (use_tma) {
+        if constexpr (Cfg::EPI == EPI_GATED) {
+          // The host lets the registers hold the whole reduction, so this is the tile's only flush: acc[0 .. CW/2) is
+          // G, acc[CW/2 .. CW) is U of the same hidden units.
+          constexpr int HW = CW / 2;
+          const int r0 = w.row0 + q * 32;
+          auto put = [&](const CUtensorMap* map, int first_acc, int c0) {   // one 32x32 piece through the staging tile
+            const uint32_t stg = stg0 + ((sbufs == 2u) ? (pc & 1u) : 0u) * Cfg::STAGING_TILE;
+            if (lane == 0) {
+              if (sbufs == 2u) tma_store_wait_read_1(); else tma_store_wait_read();
+            }
+            __syncwarp();
+#pragma unroll
+            for (int cq = 0; cq < 8; ++cq)
+              sts128(stg + lane * 128 + ((cq ^ (lane & 7)) * 16),
+                     make_float4(acc[first_acc + cq * 4], acc[first_acc + cq * 4 + 1], acc[first_acc + cq * 4 + 2],
+                                 acc[first_acc + cq * 4 + 3]));
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(map, stg, c0, r0, w.zc);
+              tma_store_commit();
+            }
+            ++pc;
+          };
+          if (p.gated_save) {
+#pragma unroll
+            for (int g = 0; g < HW / 32; ++g) {
+              const int c0 = w.col0 + h * HW + g * 32;
+              if (c0 < p.N && r0 < p.M) {   // warp-uniform
+                put(&p.tmRep[0], g * 32, c0);
+                put(&p.tmRep[1], HW + g * 32, c0);
+              }
+            }
+          }
+          gated_forward<HW>(p.act, acc);
+#pragma unroll
+          for (int g = 0; g < HW / 32; ++g) {
+            const int c0 = w.col0 + h * HW + g * 32;
+            if (c0 < p.N && r0 < p.M) put(&p.tmC, g * 32, c0);
+          }
+        } else if constexpr (Cfg::EPI == EPI_DGATED) {
+          // deltaH never leaves the SM: each 32x32 piece goes through the staging tile so that eight lanes share a
+          // row's 128 bytes (whole segments of G, U, deltaG and deltaU), and the elementwise part happens there.
+          const uint32_t stg = stg0;
+          const int sub = lane >> 3, chunk = lane & 7;
+#pragma unroll
+          for (int g = 0; g < CW / 32; ++g) {
+            const int c0 = w.col0 + h * CW + g * 32;
+            if (c0 < p.N && w.row0 + q * 32 < p.M) {   // warp-uniform
+#pragma unroll
+              for (int cq = 0; cq < 8; ++cq)
+                sts128(stg + lane * 128 + ((cq ^ (lane & 7)) * 16),
+                       make_float4(acc[g * 32 + cq * 4], acc[g * 32 + cq * 4 + 1], acc[g * 32 + cq * 4 + 2],
+                                   acc[g * 32 + cq * 4 + 3]));
+              __syncwarp();
+              const bool col_ok = c0 + chunk * 4 < p.N;   // p.N is a multiple of 4: a vector is whole or absent
+              const long long off0 = static_cast<long long>(w.row0 + q * 32 + sub) * p.ldc + c0 + chunk * 4;
+#pragma unroll
+              for (int i0 = 0; i0 < 8; i0 += 2) {
+                float4 gv[2], uv[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const int r = (i0 + i) * 4 + sub;
+                  if (col_ok && w.row0 + q * 32 + r < p.M) {
+                    const long long off = off0 + static_cast<long long>(i0 + i) * 4 * p.ldc;
+                    gv[i] = *reinterpret_cast<const float4*>(p.ep_g + off);
+                    uv[i] = *reinterpret_cast<const float4*>(p.ep_u + off);
+                  }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const int r = (i0 + i) * 4 + sub;
+                  if (col_ok && w.row0 + q * 32 + r < p.M) {
+                    const long long off = off0 + static_cast<long long>(i0 + i) * 4 * p.ldc;
+                    const float4 d = lds128(stg + r * 128 + ((chunk ^ (r & 7)) * 16));
+                    float4 dg, du;
+                    gated_backward4(p.act, d, gv[i], uv[i], &dg, &du);
+                    *reinterpret_cast<float4*>(p.ep_dg + off) = dg;
+                    *reinterpret_cast<float4*>(p.ep_du + off) = du;
+                  }
+                }
+              }
+              __syncwarp();   // the piece has been read before the next one overwrites it
+            }
+          }
+        } else if (use_tma) {
           // Each drain warp owns a 32-row x CW-column block.  32x32 pieces go through a
           // swizzled 4 KB staging tile (row r, 16-byte chunk c at r*128 + ((c ^ (r & 7)) * 16):
           // conflict-free for the row-per-lane writes) and leave as one TMA store each, which

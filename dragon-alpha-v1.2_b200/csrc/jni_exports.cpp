@@ -14,9 +14,11 @@ static inline jint jni_Throw(JNIEnv* env, jthrowable o) { return env->Throw(o); 
 static inline jobject jni_NewObjectA(JNIEnv* env, jclass c, jmethodID m, const jvalue* a) { return env->NewObjectA(c, m, a); }
 static inline jmethodID jni_GetMethodID(JNIEnv* env, jclass c, const char* n, const char* s) { return env->GetMethodID(c, n, s); }
 static inline void jni_GetLongArrayRegion(JNIEnv* env, jlongArray a, jint s, jint l, jlong* b) { env->GetLongArrayRegion(a, s, l, b); }
+static inline jint jni_GetArrayLength(JNIEnv* env, jarray a) { return env->GetArrayLength(a); }
 #else
 #include "jni_min.h"
 #endif
+#include <cstdlib>
 #include "../../include/dragon_cu32.h"
 
 namespace {
@@ -329,6 +331,89 @@ BMM_SCALED(batchMatMul_1scaled, cu32_batchMatMul_scaled)
 BMM_SCALED(batchMatMulT1_1scaled, cu32_batchMatMulT1_scaled)
 BMM_SCALED(batchMatMulT2_1scaled, cu32_batchMatMulT2_scaled)
 BMM_SCALED(batchMatMulT2_1softmax, cu32_batchMatMulT2_softmax)
+
+// ---- operators of transformer layers (no counterpart in the reference's Java classes); a class would declare
+//   Cuda_gatedFF:      public static native void gatedFF(long[] streamArray, int length, long dX, long dWg, long dWu,
+//                        long dWd, long dG, long dU, long dH, long dY, long dWork, long work_floats, int N, int D, int F,
+//                        int act);   gatedFF_delta likewise;   public static native long work(int N, int D, int F);
+//   Cuda_normResidual: normResidual, normResidual_delta (a stream handle first), work(int N, int M, int gate_rows)
+//   Cuda_gradClip:     gradNorm(long stream, long[] src, long[] sizes, int count, long dResult, long dWork, long doubles),
+//                        gradClip(... src, long[] dst, long[] sizes, int count, float max_norm, ...), work(int count)
+JNIEXPORT void JNICALL JNAME(gatedFF, gatedFF)(JNIEnv* env, jclass, jlongArray streams, jint length, jlong dX, jlong dWg,
+                                               jlong dWu, jlong dWd, jlong dG, jlong dU, jlong dH, jlong dY, jlong dWork,
+                                               jlong work_floats, jint N, jint D, jint F, jint act) {
+  Streams s(env, streams, length);
+  done(env, cu32_gatedFF(s.h, s.n, cptr(dX), cptr(dWg), cptr(dWu), cptr(dWd), mptr(dG), mptr(dU), mptr(dH), mptr(dY),
+                         mptr(dWork), work_floats, N, D, F, act));
+}
+JNIEXPORT void JNICALL JNAME(gatedFF, gatedFF_1delta)(JNIEnv* env, jclass, jlongArray streams, jint length, jlong d_deltaY,
+                                                      jlong dX, jlong dWg, jlong dWu, jlong dWd, jlong dG, jlong dU,
+                                                      jlong dH, jlong d_deltaG, jlong d_deltaU, jlong d_deltaX,
+                                                      jlong d_deltaWg, jlong d_deltaWu, jlong d_deltaWd, jlong dWork,
+                                                      jlong work_floats, jint N, jint D, jint F, jint act) {
+  Streams s(env, streams, length);
+  done(env, cu32_gatedFF_delta(s.h, s.n, cptr(d_deltaY), cptr(dX), cptr(dWg), cptr(dWu), cptr(dWd), cptr(dG), cptr(dU),
+                               cptr(dH), mptr(d_deltaG), mptr(d_deltaU), mptr(d_deltaX), mptr(d_deltaWg), mptr(d_deltaWu),
+                               mptr(d_deltaWd), mptr(dWork), work_floats, N, D, F, act));
+}
+JNIEXPORT jlong JNICALL JNAME(gatedFF, work)(JNIEnv*, jclass, jint N, jint D, jint F) { return cu32_gatedFF_work(N, D, F); }
+
+JNIEXPORT void JNICALL JNAME(normResidual, normResidual)(JNIEnv* env, jclass, jlong stream, jlong dB, jlong dR, jlong dGate,
+                                                         jint gate_rows, jlong dWpost, jlong dWpre, jlong dRout, jlong dY,
+                                                         jlong dRstdPost, jlong dRstdPre, jint N, jint M, jint width,
+                                                         jfloat res_scale, jfloat scale, jfloat eps) {
+  done(env, cu32_normResidual(stream, cptr(dB), cptr(dR), cptr(dGate), gate_rows, cptr(dWpost), cptr(dWpre), mptr(dRout),
+                              mptr(dY), mptr(dRstdPost), mptr(dRstdPre), N, M, width, res_scale, scale, eps));
+}
+JNIEXPORT void JNICALL JNAME(normResidual, normResidual_1delta)(
+    JNIEnv* env, jclass, jlong stream, jlong d_deltaRout, jlong d_deltaY, jlong dB, jlong dRout, jlong dGate, jint gate_rows,
+    jlong dWpost, jlong dWpre, jlong dRstdPost, jlong dRstdPre, jlong d_deltaR, jlong d_deltaB, jlong d_deltaGate,
+    jlong d_deltaWpost, jlong d_deltaWpre, jlong dWork, jlong work_floats, jint N, jint M, jint width, jfloat res_scale,
+    jfloat scale) {
+  done(env, cu32_normResidual_delta(stream, cptr(d_deltaRout), cptr(d_deltaY), cptr(dB), cptr(dRout), cptr(dGate), gate_rows,
+                                    cptr(dWpost), cptr(dWpre), cptr(dRstdPost), cptr(dRstdPre), mptr(d_deltaR),
+                                    mptr(d_deltaB), mptr(d_deltaGate), mptr(d_deltaWpost), mptr(d_deltaWpre), mptr(dWork),
+                                    work_floats, N, M, width, res_scale, scale));
+}
+JNIEXPORT jlong JNICALL JNAME(normResidual, work)(JNIEnv*, jclass, jint N, jint M, jint gate_rows) {
+  return cu32_normResidual_work(N, M, gate_rows);
+}
+
+namespace {
+// The first `count` elements of a long[]; `rc` is set where the array is null or shorter, or the host has no memory.
+struct Longs {
+  jlong* v = nullptr;
+  Longs(JNIEnv* env, jlongArray arr, jint count, int* rc) {
+    if (*rc) return;
+    if (!arr) { *rc = CU32_E_NULL; return; }
+    if (count <= 0 || jni_GetArrayLength(env, arr) < count) { *rc = CU32_E_DIM; return; }
+    v = static_cast<jlong*>(std::malloc(sizeof(jlong) * static_cast<size_t>(count)));
+    if (!v) { *rc = 2; return; }     // cudaErrorMemoryAllocation
+    jni_GetLongArrayRegion(env, arr, 0, count, v);
+  }
+  ~Longs() { std::free(v); }
+  Longs(const Longs&) = delete;
+  const int64_t* get() const { return reinterpret_cast<const int64_t*>(v); }
+};
+inline double* dptr(jlong a) { return reinterpret_cast<double*>(static_cast<intptr_t>(a)); }
+}  // namespace
+JNIEXPORT void JNICALL JNAME(gradClip, gradNorm)(JNIEnv* env, jclass, jlong stream, jlongArray src, jlongArray sizes,
+                                                 jint count, jlong dResult, jlong dWork, jlong work_doubles) {
+  int rc = 0;
+  Longs a(env, src, count, &rc), z(env, sizes, count, &rc);
+  if (!rc) rc = cu32_gradNorm(stream, a.get(), z.get(), count, mptr(dResult), dptr(dWork), work_doubles);
+  done(env, rc);
+}
+JNIEXPORT void JNICALL JNAME(gradClip, gradClip)(JNIEnv* env, jclass, jlong stream, jlongArray src, jlongArray dst,
+                                                 jlongArray sizes, jint count, jfloat max_norm, jlong dResult, jlong dWork,
+                                                 jlong work_doubles) {
+  int rc = 0;
+  Longs a(env, src, count, &rc), b(env, dst, count, &rc), z(env, sizes, count, &rc);
+  if (!rc)
+    rc = cu32_gradClip(stream, a.get(), b.get(), z.get(), count, max_norm, mptr(dResult), dptr(dWork), work_doubles);
+  done(env, rc);
+}
+JNIEXPORT jlong JNICALL JNAME(gradClip, work)(JNIEnv*, jclass, jint count) { return cu32_gradClip_work(count); }
 
 // ---- Cuda_dconv3D_deltaW (Java declarations: Cuda_dconv3D_deltaW.java:288-640)
 #define JNAME_DW(method) Java_z_dragon_engine_cuda_impl_math_Cuda_1dconv3D_1deltaW_##method

@@ -59,6 +59,10 @@ static inline void jni_GetLongArrayRegion(JNIEnv* env, jlongArray arr, jint star
   reinterpret_cast<Fn>((*env)->slot[204])(env, arr, start, len, buf);
 }
 
+static inline jint jni_GetArrayLength(JNIEnv* env, jarray arr) {
+  typedef jint (*Fn)(JNIEnv*, jarray);
+  return reinterpret_cast<Fn>((*env)->slot[171])(env, arr);
+}
 static inline jstring jni_NewStringUTF(JNIEnv* env, const char* utf) {
   typedef jstring (*Fn)(JNIEnv*, const char*);
   return reinterpret_cast<Fn>((*env)->slot[167])(env, utf);

@@ -13,6 +13,7 @@ says how to build it.
 from __future__ import annotations
 
 import ctypes
+from array import array
 from ctypes import c_char_p, c_float, c_int, c_int64, POINTER
 from pathlib import Path
 
@@ -53,6 +54,8 @@ def _sig(lib, name, argtypes):
 
 # name -> ctypes argument types; also the list of symbols include/dragon_cu32.h declares.
 _I = c_int
+_vp = ctypes.c_void_p
+_ll = ctypes.c_longlong
 SIGNATURES = {
     "cu32_matMul": [_sp, _I, _fp, _fp, _fp, _I, _I, _I],
     "cu32_matMulT1": [_sp, _I, _fp, _fp, _fp, _I, _I, _I],
@@ -137,6 +140,16 @@ SIGNATURES = {
     "cu32_conv3D_texture": [_sp, _I, _fp, _I, _I, _fp, _I, _I, _fp] + [_I] * 9,
     "cu32_conv3D_np": [_sp, _I, _fp, _I, _I, _fp, _I, _I, _fp] + [_I] * 7,
     "cu32_conv3D_W1": [_sp, _I, _fp, _I, _I, _fp, _fp, _I, _I, _I],
+    # device addresses as plain integers (no cast per argument: these calls are short)
+    "cu32_gatedFF": [_sp, _I] + [_vp] * 9 + [_ll] + [_I] * 4,
+    "cu32_gatedFF_delta": [_sp, _I] + [_vp] * 15 + [_ll] + [_I] * 4,
+    "cu32_normResidual": [c_int64, _vp, _vp, _vp, _I, _vp, _vp, _vp, _vp, _vp, _vp, _I, _I, _I, c_float, c_float, c_float],
+    "cu32_normResidual_delta": [c_int64] + [_vp] * 5 + [_I] + [_vp] * 10 + [_ll, _I, _I, _I, c_float, c_float],
+    "cu32_gradNorm": [c_int64, _vp, _vp, _I, _vp, _vp, _ll],
+    "cu32_gradClip": [c_int64, _vp, _vp, _vp, _I, c_float, _vp, _vp, _ll],
+    "cu32_gatedFF_work": [_I, _I, _I],
+    "cu32_normResidual_work": [_I, _I, _I],
+    "cu32_gradClip_work": [_I],
     "cu32_tune": [c_char_p, _I],
     "cu32_get_tune": [c_char_p, POINTER(c_int)],
     "cu32_read_status": [POINTER(c_int)],
@@ -157,6 +170,8 @@ def load():
     lib = ctypes.CDLL(str(LIB_PATH))
     for name, args in SIGNATURES.items():
         _sig(lib, name, args)
+        if name.endswith("_work"):      # scratch sizes: a count, not a status
+            getattr(lib, name).restype = ctypes.c_longlong
     lib.cu32_version.argtypes = []
     lib.cu32_version.restype = c_char_p
     _lib = lib
@@ -755,3 +770,86 @@ class Cuda_dconv3D_deltaW:
     @staticmethod
     def Im2col_WinogradV2_SHW_s16_texture(streamArray, length, GridZ, OH_slice, OW_slice, c64, *a):
         return Cuda_dconv3D_deltaW._wino("s16_texture", (c64,), streamArray, length, GridZ, OH_slice, OW_slice, *a)
+
+
+class Cuda_gatedFF:
+    """Gated feed-forward block H = act(X Wg) * (X Wu), Y = H Wd and its gradients (no counterpart among the reference's
+    natives).  X [N, D], Wg and Wu [D, F], Wd [F, D], D and F multiples of 4; addresses are integers, 0 = null."""
+
+    SILU, GELU, GELU_TANH, RELU, SIGMOID = range(5)
+
+    @staticmethod
+    def work(N, D, F) -> int:
+        """Floats of scratch that let every product of the two calls be split as far as it would."""
+        return load().cu32_gatedFF_work(N, D, F)
+
+    @staticmethod
+    def gatedFF(streamArray, length, dX, dWg, dWu, dWd, dG, dU, dH, dY, dWork, work_floats, N, D, F, act):
+        """Writes H and Y; G = X Wg and U = X Wu as well where they are given (training)."""
+        s, n = _streams(streamArray, length)
+        _check(load().cu32_gatedFF(s, n, dX, dWg, dWu, dWd, dG, dU, dH, dY, dWork, work_floats, N, D, F, act), "gatedFF")
+
+    @staticmethod
+    def gatedFF_delta(streamArray, length, d_deltaY, dX, dWg, dWu, dWd, dG, dU, dH, d_deltaG, d_deltaU, d_deltaX,
+                      d_deltaWg, d_deltaWu, d_deltaWd, dWork, work_floats, N, D, F, act):
+        """deltaG and deltaU always (they may replace G and U), the others where they are given."""
+        s, n = _streams(streamArray, length)
+        _check(load().cu32_gatedFF_delta(s, n, d_deltaY, dX, dWg, dWu, dWd, dG, dU, dH, d_deltaG, d_deltaU, d_deltaX,
+                                         d_deltaWg, d_deltaWu, d_deltaWd, dWork, work_floats, N, D, F, act),
+               "gatedFF_delta")
+
+
+class Cuda_normResidual:
+    """RMS norms before and after a block fused with its gate and the residual's scale (no counterpart among the
+    reference's natives): P = w_post * B / rms(B), R' = res_scale * R + scale * gate * P, Y = w_pre * R' / rms(R')."""
+
+    @staticmethod
+    def work(N, M, gate_rows) -> int:
+        """Floats of scratch for normResidual_delta."""
+        return load().cu32_normResidual_work(N, M, gate_rows)
+
+    @staticmethod
+    def normResidual(stream, dB, dR, dGate, gate_rows, dWpost, dWpre, dRout, dY, dRstdPost, dRstdPre, N, M, width,
+                     res_scale, scale, eps):
+        _check(load().cu32_normResidual(stream, dB, dR, dGate, gate_rows, dWpost, dWpre, dRout, dY, dRstdPost, dRstdPre,
+                                        N, M, width, res_scale, scale, eps), "normResidual")
+
+    @staticmethod
+    def normResidual_delta(stream, d_deltaRout, d_deltaY, dB, dRout, dGate, gate_rows, dWpost, dWpre, dRstdPost, dRstdPre,
+                           d_deltaR, d_deltaB, d_deltaGate, d_deltaWpost, d_deltaWpre, dWork, work_floats, N, M, width,
+                           res_scale, scale):
+        _check(load().cu32_normResidual_delta(stream, d_deltaRout, d_deltaY, dB, dRout, dGate, gate_rows, dWpost, dWpre,
+                                              dRstdPost, dRstdPre, d_deltaR, d_deltaB, d_deltaGate, d_deltaWpost,
+                                              d_deltaWpre, dWork, work_floats, N, M, width, res_scale, scale),
+               "normResidual_delta")
+
+
+class Cuda_gradClip:
+    """Global norm of many gradient tensors and clipping (no counterpart among the reference's natives).  Addresses and
+    sizes are sequences of integers; an ``array.array('q')`` is passed as it is."""
+
+    @staticmethod
+    def _ints(values, count):
+        a = values if isinstance(values, array) and values.typecode == "q" else array("q", values)
+        if len(a) < count:
+            raise ValueError(f"{count} tensors, but a sequence of {len(a)}")
+        return a
+
+    @staticmethod
+    def work(count) -> int:
+        """Doubles of scratch for `count` tensors."""
+        return load().cu32_gradClip_work(count)
+
+    @staticmethod
+    def gradNorm(stream, src, sizes, count, dResult, dWork, work_doubles):
+        """dResult[0] = norm, dResult[1] = 1."""
+        a, z = Cuda_gradClip._ints(src, count), Cuda_gradClip._ints(sizes, count)
+        _check(load().cu32_gradNorm(stream, a.buffer_info()[0], z.buffer_info()[0], count, dResult, dWork, work_doubles),
+               "gradNorm")
+
+    @staticmethod
+    def gradClip(stream, src, dst, sizes, count, max_norm, dResult, dWork, work_doubles):
+        """dst = src * min(1, max_norm / norm); dResult = {norm, factor}."""
+        a, b, z = (Cuda_gradClip._ints(v, count) for v in (src, dst, sizes))
+        _check(load().cu32_gradClip(stream, a.buffer_info()[0], b.buffer_info()[0], z.buffer_info()[0], count, max_norm,
+                                    dResult, dWork, work_doubles), "gradClip")

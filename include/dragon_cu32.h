@@ -426,6 +426,83 @@ CU32_API int cu32_conv3D_GemmR_biased(const int64_t* streams, int length, const 
 CU32_API int cu32_batchMatMulT2_softmax(const int64_t* streams, int length, const float* dA, const float* dB,
                                         float* dP, int Batch, int N, int CM, int BM, int K, float alpha);
 
+/* ------------------------------------------------------------------ gated feed-forward block
+ * H = act(X Wg) * (X Wu), Y = H Wd, and its gradients.  No counterpart among the reference's natives (its engine would
+ * run three products and elementwise kernels).
+ *   X [N, D]; Wg, Wu [D, F]; Wd [F, D]; G = X Wg, U = X Wu, H [N, F]; Y [N, D]; D and F multiples of 4, any N >= 1;
+ *   every base pointer 16-byte aligned.  act: one of CU32_ACT_*, applied to G.
+ * cu32_gatedFF
+ *   G and U are written for the gradient call when given; both null in serving.  H is always written.
+ *   Up to 16 rows the weights are read once for all rows (FP32 multiply-adds); more rows run on the tensor cores, both
+ *   projections, the activation and the product in one kernel.
+ * cu32_gatedFF_delta
+ *   deltaH = deltaY Wd^T, deltaG = deltaH * U * act'(G), deltaU = deltaH * act(G), both written (dG may be G and dU may
+ *   be U: they are then replaced); deltaX = deltaG Wg^T + deltaU Wu^T, deltaWg = X^T deltaG, deltaWu = X^T deltaU,
+ *   deltaWd = H^T deltaY.  deltaX, deltaWg, deltaWu and deltaWd may each be null: that gradient is not computed (and
+ *   the operands only it needs may be null).
+ * work: work_floats floats of scratch for split reductions, or null / 0 (products are then not split); its contents
+ *   mean nothing between calls, and calls that may overlap need scratch of their own.  cu32_gatedFF_work says how many
+ *   floats let every product of the two calls split as far as it would.
+ * All outputs are fully overwritten; results do not vary from run to run (no atomics).  An infinite pre-activation
+ * gives what the formula gives (NaN for SILU at -inf). */
+#define CU32_ACT_SILU 0        /* x / (1 + e^-x) */
+#define CU32_ACT_GELU 1        /* x Phi(x) */
+#define CU32_ACT_GELU_TANH 2   /* x / (1 + e^(-2 z)), z = sqrt(2/pi) (x + 0.044715 x^3) */
+#define CU32_ACT_RELU 3
+#define CU32_ACT_SIGMOID 4
+CU32_API int cu32_gatedFF(const int64_t* streams, int length, const float* dX, const float* dWg, const float* dWu,
+                          const float* dWd, float* dG, float* dU, float* dH, float* dY, float* dWork,
+                          long long work_floats, int N, int D, int F, int act);
+CU32_API int cu32_gatedFF_delta(const int64_t* streams, int length, const float* d_deltaY, const float* dX,
+                                const float* dWg, const float* dWu, const float* dWd, const float* dG, const float* dU,
+                                const float* dH, float* d_deltaG, float* d_deltaU, float* d_deltaX, float* d_deltaWg,
+                                float* d_deltaWu, float* d_deltaWd, float* dWork, long long work_floats, int N, int D,
+                                int F, int act);
+CU32_API long long cu32_gatedFF_work(int N, int D, int F);
+
+/* ------------------------------------------------------------------ norms around a block, gate and residual scale
+ * For every row of `width` columns (pitch M floats, a multiple of 4, at most 16384; columns >= width are ignored on the
+ * way in and written as zeros):
+ *   rms(x) = sqrt(mean(x^2) + eps);   P = w_post * B / rms(B), or B where w_post is null
+ *   R' = res_scale * R + scale * gate * P;   Y = w_pre * R' / rms(R')
+ * B: what the block computed, R: the residual it read, Y: what the next block reads.  No counterpart among the
+ * reference's natives.
+ *   gate: null, or [ceil(N / gate_rows), M]; its row g serves the rows g * gate_rows ... (gate_rows = N: one per channel;
+ *   the length of a sequence: one per sequence; 1: one per row).
+ *   rstd_post, rstd_pre [N]: 1 / rms(B), 1 / rms(R') for the gradient call, or null.
+ *   Rout may be R (the residual is then replaced), Y may be B.
+ * cu32_normResidual_delta: from deltaRout (null = 0) and deltaY the gradients deltaR, deltaB, deltaGate (as gate),
+ *   deltaWpost and deltaWpre [M]; the outputs of operands that were null are not touched and may be null.  deltaR may
+ *   be deltaRout or deltaY, deltaB the other.  work: cu32_normResidual_work floats of scratch
+ *   (fewer, down to 3 M, run with fewer thread blocks; below that CU32_E_SCRATCH).
+ * Results do not vary from run to run (no atomics).  eps >= 0; with eps = 0 a row of zeros gives NaN. */
+CU32_API int cu32_normResidual(int64_t stream, const float* dB, const float* dR, const float* dGate, int gate_rows,
+                               const float* dWpost, const float* dWpre, float* dRout, float* dY, float* dRstdPost,
+                               float* dRstdPre, int N, int M, int width, float res_scale, float scale, float eps);
+CU32_API long long cu32_normResidual_work(int N, int M, int gate_rows);
+CU32_API int cu32_normResidual_delta(int64_t stream, const float* d_deltaRout, const float* d_deltaY, const float* dB,
+                                     const float* dRout, const float* dGate, int gate_rows, const float* dWpost,
+                                     const float* dWpre, const float* dRstdPost, const float* dRstdPre, float* d_deltaR,
+                                     float* d_deltaB, float* d_deltaGate, float* d_deltaWpost, float* d_deltaWpre,
+                                     float* dWork, long long work_floats, int N, int M, int width, float res_scale,
+                                     float scale);
+
+/* ------------------------------------------------------------------ global gradient norm and clipping
+ * norm = sqrt(sum of g^2 over all tensors), squares and sums in 64 bits; factor = max_norm / norm where norm > max_norm,
+ * else 1; dst = src * factor.  No counterpart among the reference's natives.
+ *   src, dst: host arrays of `count` device addresses (4-byte aligned; dst[i] may be src[i], anything else must not
+ *   overlap), sizes: host array of their float counts (0 allowed).  The arrays are read during the call only.
+ *   result: two device floats, {norm, factor}.  A tensor that stays in place is not touched where the factor is 1.
+ *   A norm that is not finite (an infinity or NaN among the gradients) gives factor 1: nothing is scaled, and the caller
+ *   sees the norm.  max_norm >= 0 (infinity allowed).
+ *   work: cu32_gradClip_work(count) device doubles of scratch; calls that may overlap need scratch of their own.
+ * The norm does not vary from run to run.  cu32_gradNorm computes the norm alone (factor 1). */
+CU32_API long long cu32_gradClip_work(int count);
+CU32_API int cu32_gradNorm(int64_t stream, const int64_t* src, const int64_t* sizes, int count, float* dResult,
+                           double* dWork, long long work_doubles);
+CU32_API int cu32_gradClip(int64_t stream, const int64_t* src, const int64_t* dst, const int64_t* sizes, int count,
+                           float max_norm, float* dResult, double* dWork, long long work_doubles);
+
 /* ------------------------------------------------------------------ library control
  * No counterpart in the reference (its only native-side switch is a compile-time macro). */
 
