@@ -26,6 +26,7 @@ struct TensorList {
   long long size[CAP];
   int first[CAP + 1];
   int count;
+  int in_place;           // every tensor's destination is its source
 };
 
 template <int CAP>
@@ -99,6 +100,7 @@ __global__ void __launch_bounds__(THREADS) grad_clip_kernel(const __grid_constan
     result[0] = static_cast<float>(norm);
     result[1] = factor;
   }
+  if (!clip && list.in_place) return;
   const int chunks = list.first[list.count];
   for (int c = chunks - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {
     const int t = tensor_of(list, c);
@@ -112,13 +114,19 @@ __global__ void __launch_bounds__(THREADS) grad_clip_kernel(const __grid_constan
       const int vecs = (n - head) >> 2;
       const float4* gv = reinterpret_cast<const float4*>(g + head);
       float4* ov = reinterpret_cast<float4*>(out + head);
+      // all loads before the first store: source and destination may be the same, so the compiler cannot reorder them
+      float4 x[CHUNK / 4 / THREADS];
+#pragma unroll
+      for (int i = 0; i < CHUNK / 4 / THREADS; ++i) {
+        const int v = i * THREADS + threadIdx.x;
+        if (v < vecs) x[i] = gv[v];
+      }
 #pragma unroll
       for (int i = 0; i < CHUNK / 4 / THREADS; ++i) {
         const int v = i * THREADS + threadIdx.x;
         if (v < vecs) {
-          float4 x = gv[v];
-          if (clip) { x.x *= factor; x.y *= factor; x.z *= factor; x.w *= factor; }   // a copy keeps every bit
-          ov[v] = x;
+          if (clip) { x[i].x *= factor; x[i].y *= factor; x[i].z *= factor; x[i].w *= factor; }   // a copy keeps every bit
+          ov[v] = x[i];
         }
       }
       const int tail = head + vecs * 4;
@@ -142,6 +150,7 @@ template <int CAP>
 int fill_list(TensorList<CAP>* list, const int64_t* src, const int64_t* dst, const int64_t* sizes, int from, int count) {
   list->count = 0;
   list->first[0] = 0;
+  list->in_place = 1;
   int i = from;
   for (; i < count && list->count < CAP; ++i) {
     if (sizes[i] == 0) continue;
@@ -150,6 +159,7 @@ int fill_list(TensorList<CAP>* list, const int64_t* src, const int64_t* dst, con
     const int t = list->count++;
     list->src[t] = reinterpret_cast<const float*>(static_cast<intptr_t>(src[i]));
     list->dst[t] = dst ? reinterpret_cast<float*>(static_cast<intptr_t>(dst[i])) : nullptr;
+    if (!dst || dst[i] != src[i]) list->in_place = 0;
     list->size[t] = sizes[i];
     list->first[t + 1] = list->first[t] + static_cast<int>(chunks);
   }

@@ -16,10 +16,10 @@
 //
 // Bound by memory: forward 4 floats per element (B, R in; R', Y out), gradients 6 (four in, two out).  Few rows: a block
 // per row, everything at once in its registers.  Many rows: persistent blocks (clusters of two or four for rows of more
-// than 4096 columns, each block a part of the row) with a producer warp that brings the next rows into a ring in shared
-// memory by bulk copies while the others compute, so that loads are in flight all the time whatever the row's
-// reductions wait for.  The column sums are kept in registers over all rows of a block, written once per block and added
-// in a fixed order by a second, small kernel (no atomics: results do not vary from run to run).
+// than 4096 columns, each block a part of the row) that keep a ring of rows in shared memory filled by bulk copies: a row
+// moves to registers in one step and its place is refilled at once, so that two rows or more are on their way whatever
+// the row in hand waits for.  The column sums are kept in registers over all rows of a block, written once per block
+// and added in a fixed order by a second, small kernel (no atomics: results do not vary from run to run).
 #include <atomic>
 
 #include "cu32_host.h"
@@ -30,7 +30,11 @@ namespace {
 using namespace ptx;
 
 constexpr int MAX_WIDTH = 16384;     // floats per row: a cluster of four blocks of 1024 vectors
-constexpr int VPT = 2;               // 16-byte vectors per thread of the persistent kernels
+// 16-byte vectors per thread of the persistent kernels.  Two, so that the weights fit in the registers beside the sums: a
+// ring that fills the shared memory leaves the L1 cache too little for 48 KB of weights, and reading them from L2 for
+// every row made the kernels wait for it (with four per thread: 145 us forward, 213 us gradients at 8192 x 4096).
+constexpr int VPT = 2;
+constexpr int RING_THREADS = 512;
 
 __device__ __forceinline__ float4 ldg_row(const float* p) {       // read once: not kept in L1
   float4 v;
@@ -54,6 +58,11 @@ __device__ __forceinline__ float4 ones4() { return make_float4(1.f, 1.f, 1.f, 1.
 __device__ __forceinline__ float square_sum(float4 v) { return v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w; }
 __device__ __forceinline__ float4 scaled(float4 v, float f, float4 w) {
   return make_float4(v.x * f * w.x, v.y * f * w.y, v.z * f * w.z, v.w * f * w.w);
+}
+// 1 / sqrt(x): the hardware's estimate and one Newton step (0 and infinity have no step)
+__device__ __forceinline__ float inv_root(float x) {
+  const float r = rsqrtf(x);
+  return x > 0.0f && x < INFINITY ? r * fmaf(-0.5f * x * r, r, 1.5f) : r;
 }
 // vector v of a row of weights, columns >= width as 0
 __device__ __forceinline__ float4 load_weight(const float* w, int v, int width) {
@@ -80,20 +89,20 @@ struct BlockSum {
   }
 };
 
-// Sums of K values over the working warps of the blocks of a cluster, in two steps: post() publishes this warp's sums and
-// returns at once, wait() delivers the totals of the oldest posted set.  Two sets may be open (the slots alternate): a
-// warp posts set i + 2 only after its wait for set i + 1, which every warp posted after it had read set i.
+// Sums of K values over the warps of a cluster's blocks, the same in every thread; false when a wait ran out.  The slots
+// alternate: a slot is written again only after its writer has waited for the set in between, which every warp delivered
+// after it had read the slot.
 template <int K, int CL>
 struct TeamSum {
-  float (*slots)[K][64];      // [2][K][64]: by set parity, value, warp of the cluster (at most 16 per block)
-  uint64_t* bars;             // [2], one arrival per warp of the cluster
+  float (*slots)[K][64];      // [2][K][64]: by set, value, warp of the cluster (at most 16 per block); zeroed at the start
+  uint64_t* bars;             // [2]
   volatile int* abort_flag;
-  int warps;                  // working warps per block
-  uint32_t posted = 0, taken = 0;
+  uint32_t sets = 0;
 
-  __device__ __forceinline__ void post(float (&v)[K]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int par = posted & 1;
+  __device__ __forceinline__ bool operator()(float (&v)[K]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int par = sets & 1;
+    const uint32_t bar = smem_u32(&bars[par]);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -102,33 +111,34 @@ struct TeamSum {
       if (lane == 0) {
 #pragma unroll
         for (int k = 0; k < K; ++k) slots[par][k][warp] = v[k];
-        mbar_arrive(smem_u32(&bars[par]));
+        mbar_arrive(bar);
       }
-    } else if (lane < CL) {     // lane r delivers to block r
-      const int at = static_cast<int>(cluster_ctarank()) * warps + warp;
+    } else {
+      // Lane r delivers to block r; each value carries its own count to that block's barrier.  (An arrival that
+      // releases at cluster scope would first wait for this thread's global stores: twice the row's time.)
+      if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(warps * CL * K * 4));
+      if (lane < CL) {
+        const int at = static_cast<int>(cluster_ctarank()) * warps + warp;
+        const uint32_t there = mapa(bar, lane);
 #pragma unroll
-      for (int k = 0; k < K; ++k) st_cluster(mapa(smem_u32(&slots[par][k][at]), lane), v[k]);
-      mbar_arrive_cluster_release(mapa(smem_u32(&bars[par]), lane));
+        for (int k = 0; k < K; ++k) st_async(mapa(smem_u32(&slots[par][k][at]), lane), v[k], there);
+      }
     }
-    ++posted;
-  }
-  __device__ __forceinline__ bool wait(float (&v)[K]) {
-    const int lane = threadIdx.x & 31;
-    const int par = taken & 1;
-    if (!mbar_wait<(CL > 1)>(smem_u32(&bars[par]), (taken >> 1) & 1u, abort_flag)) return false;
+    if (!mbar_wait(bar, (sets >> 1) & 1u, abort_flag)) return false;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float x = lane < warps * CL ? slots[par][k][lane] : 0.0f;
-      if (CL > 2 && lane + 32 < warps * CL) x += slots[par][k][lane + 32];
+      float x = slots[par][k][CL == 1 ? lane & 15 : lane];      // both halves of the warp add the same 16
+      if (CL > 2) x += slots[par][k][lane + 32];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      for (int o = CL == 1 ? 8 : 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
       v[k] = x;
     }
-    ++taken;
+    ++sets;
     return true;
   }
-  static __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+  static __device__ __forceinline__ void st_async(uint32_t addr, float v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+                 ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
   }
 };
 
@@ -150,13 +160,9 @@ struct NormParams {
 };
 
 // R' of one vector: res_scale R + scale gate (B rb w_post)
-__device__ __forceinline__ float4 new_residual(const NormParams& p, float4 b, float4 r, float rb, float4 wpost,
-                                               const float* gate, int v) {
+__device__ __forceinline__ float4 new_residual(const NormParams& p, float4 b, float4 r, float rb, float4 wpost, float4 gate) {
   float4 x = scaled(b, rb, wpost);
-  if (gate != nullptr) {
-    const float4 g = load_weight(gate, v, p.width);
-    x.x *= g.x; x.y *= g.y; x.z *= g.z; x.w *= g.w;
-  }
+  x.x *= gate.x; x.y *= gate.y; x.z *= gate.z; x.w *= gate.w;
   return make_float4(fmaf(p.scale, x.x, p.res_scale * r.x), fmaf(p.scale, x.y, p.res_scale * r.y),
                      fmaf(p.scale, x.z, p.res_scale * r.z), fmaf(p.scale, x.w, p.res_scale * r.w));
 }
@@ -183,7 +189,7 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const __grid_constan
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) s += square_sum(b[i]);
-    rb = 1.0f / sqrtf(fmaf(sum(s), inv_width, p.eps));
+    rb = inv_root(fmaf(sum(s), inv_width, p.eps));
     if (p.rstd_post != nullptr && threadIdx.x == 0) p.rstd_post[row] = rb;
   }
   const float* gate = p.gate == nullptr ? nullptr : p.gate + static_cast<long long>(row / p.gate_rows) * p.M;
@@ -192,12 +198,13 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const __grid_constan
   for (int i = 0; i < V; ++i) {
     const int v = i * blockDim.x + threadIdx.x;
     if (v < vecs) {
-      r[i] = new_residual(p, b[i], r[i], rb, p.wpost ? load_weight(p.wpost, v, p.width) : ones4(), gate, v);
+      r[i] = new_residual(p, b[i], r[i], rb, p.wpost ? load_weight(p.wpost, v, p.width) : ones4(),
+                          gate ? load_weight(gate, v, p.width) : ones4());
       *reinterpret_cast<float4*>(p.Rout + base + v * 4) = r[i];
       s += square_sum(r[i]);
     }
   }
-  const float rr = 1.0f / sqrtf(fmaf(sum(s), inv_width, p.eps));
+  const float rr = inv_root(fmaf(sum(s), inv_width, p.eps));
   if (p.rstd_pre != nullptr && threadIdx.x == 0) p.rstd_pre[row] = rr;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -207,11 +214,11 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const __grid_constan
 }
 
 // ------------------------------------------------------------------ ring of rows in shared memory
-constexpr int MAX_STAGES = 4;
-constexpr int ROLE_NORM_PRODUCER = 8, ROLE_NORM_ROW = 9;     // who gave up, in the status word
+constexpr int MAX_STAGES = 6;
+constexpr int ROLE_NORM_ROW = 8, ROLE_NORM_SUM = 9;     // what was waited for in vain, in the status word
 
 struct RingBars {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], team[2];
+  uint64_t full[MAX_STAGES], team[2];
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const float* src, uint32_t bytes, uint32_t bar) {
@@ -223,142 +230,151 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ void give_up(const NormParams& p, volatile int* abort_flag, int role, uint32_t it) {
-  *abort_flag = 1;
-  atomicCAS(p.status, 0, (role << 24) | static_cast<int>(it & 0xFFFF));
-}
 
-// Sets up the barriers; every thread of the cluster returns when they can be used.
-template <int CL>
-__device__ __forceinline__ void ring_setup(RingBars* bars, volatile int* abort_flag, int warps) {
+// Sets up the barriers and clears the K-value slots; every thread of the cluster returns when they can be used.
+template <int CL, int K>
+__device__ __forceinline__ void ring_setup(RingBars* bars, volatile int* abort_flag, float (*slots)[K][64]) {
+  for (int i = threadIdx.x; i < 2 * K * 64; i += blockDim.x) (&slots[0][0][0])[i] = 0.0f;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < MAX_STAGES; ++i) {
-      mbar_init(smem_u32(&bars->full[i]), 1);
-      mbar_init(smem_u32(&bars->empty[i]), warps);
-    }
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bars->team[i]), warps * CL);
+    for (int i = 0; i < MAX_STAGES; ++i) mbar_init(smem_u32(&bars->full[i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bars->team[i]), CL == 1 ? blockDim.x >> 5 : 1);
     fence_mbar_init();
   }
   __syncthreads();
   if (CL > 1) cluster_sync();
 }
 
-// One thread: copies `arrays` row parts per row into the ring, rows in the order that next() gives them (-1: the end).
-template <class Next>
-__device__ __forceinline__ void produce(const NormParams& p, RingBars* bars, volatile int* abort_flag, uint32_t ring,
-                                        const float* const (&src)[4], uint32_t part_bytes, long long part_offset, Next next) {
-  uint32_t it = 0, s = 0, ph = 0;
-  for (long long row; (row = next()) >= 0; ++it) {
-    if (!mbar_wait(smem_u32(&bars->empty[s]), ph ^ 1u, abort_flag)) {
-      give_up(p, abort_flag, ROLE_NORM_PRODUCER, it);
-      break;
-    }
-    const uint32_t bar = smem_u32(&bars->full[s]);
+// The ring of A arrays per row.  refill() is for thread 0 alone, after a team sum that every warp took part in after it
+// had read the place that is filled again.
+template <int A>
+struct Ring {
+  const NormParams& p;
+  RingBars* bars;
+  volatile int* abort_flag;
+  uint32_t base, part_bytes;
+  long long part_offset;
+  uint32_t read_at = 0, read_ph = 0, fill_at = 0, filled = 0, taken = 0;
+
+  __device__ __forceinline__ void refill(const float* const (&src)[A], int row) {
+    const uint32_t bar = smem_u32(&bars->full[fill_at]);
     uint32_t bytes = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) bytes += src[k] != nullptr ? part_bytes : 0u;
+    for (int k = 0; k < A; ++k) bytes += src[k] != nullptr ? part_bytes : 0u;
     mbar_arrive_expect_tx(bar, bytes);
+    const long long at = static_cast<long long>(row) * p.M + part_offset;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (src[k] != nullptr)
-        bulk_load(ring + s * p.stage_bytes + k * p.slab_bytes, src[k] + row * p.M + part_offset, part_bytes, bar);
-    if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1u; }
+    for (int k = 0; k < A; ++k)
+      if (src[k] != nullptr) bulk_load(base + fill_at * p.stage_bytes + k * p.slab_bytes, src[k] + at, part_bytes, bar);
+    if (++fill_at == static_cast<uint32_t>(p.stages)) fill_at = 0;
+    ++filled;
   }
-  if (*abort_flag) {     // copies in flight land before the block may leave
-    const uint32_t n = it < static_cast<uint32_t>(p.stages) ? it : static_cast<uint32_t>(p.stages);
-    for (uint32_t k = 0; k < n; ++k) {
-      const uint32_t i = it - n + k;
+  // the next row's place, once its data is there; 0 when the wait ran out
+  __device__ __forceinline__ uint32_t take() {
+    if (!mbar_wait(smem_u32(&bars->full[read_at]), read_ph, abort_flag)) return 0u;
+    const uint32_t at = base + read_at * p.stage_bytes;
+    if (++read_at == static_cast<uint32_t>(p.stages)) { read_at = 0; read_ph ^= 1u; }
+    ++taken;
+    return at;
+  }
+  // after a give-up: copies in flight land before the block may leave (thread 0, bounded)
+  __device__ __forceinline__ void land() {
+    for (; taken < filled; ++taken) {
       const long long t0 = clock64();
-      while (!mbar_try_wait(smem_u32(&bars->full[i % p.stages]), (i / p.stages) & 1u) && clock64() - t0 < 20000000LL) {
+      while (!mbar_try_wait(smem_u32(&bars->full[taken % p.stages]), (taken / p.stages) & 1u) && clock64() - t0 < 20000000LL) {
       }
     }
   }
+};
+
+__device__ __forceinline__ void give_up(const NormParams& p, volatile int* abort_flag, int role, int row) {
+  *abort_flag = 1;
+  if ((threadIdx.x & 31) == 0) atomicCAS(p.status, 0, (role << 24) | (row & 0xFFFF));
 }
 
 // ------------------------------------------------------------------ forward, many rows
-// Block: the working warps, then one producer warp.  The block (cluster) takes rows unit, unit + units, ...
+// The block (cluster) takes rows unit, unit + units, ...
 template <int CL>
-__global__ void __launch_bounds__(544) norm_forward_ring_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(RING_THREADS, 2) norm_forward_ring_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ __align__(8) RingBars bars;
   __shared__ float slots[2][1][64];
   __shared__ volatile int abort_flag;
-  const int warps = (blockDim.x >> 5) - 1;
-  ring_setup<CL>(&bars, &abort_flag, warps);
+  ring_setup<CL, 1>(&bars, &abort_flag, slots);
   const int rank = CL > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int unit = blockIdx.x / CL;
   const int vec0 = rank * p.vecs, vecs = min(p.vecs, p.M / 4 - vec0);     // this block's part of the row
-  const uint32_t ring = smem_u32(ring_smem);
-  if ((threadIdx.x >> 5) == warps) {
-    if ((threadIdx.x & 31) == 0) {
-      const float* const src[4] = {p.B, p.R, nullptr, nullptr};
-      long long row = unit - p.units;
-      produce(p, &bars, &abort_flag, ring, src, vecs * 16, vec0 * 4, [&]() -> long long {
-        row += p.units;
-        return row < p.N ? row : -1;
-      });
+  const int T = blockDim.x;
+  const bool post = p.wpost != nullptr;
+  const float* const src[2] = {p.B, p.R};
+  Ring<2> ring{p, &bars, &abort_flag, smem_u32(ring_smem), static_cast<uint32_t>(vecs * 16), vec0 * 4};
+  int fill_row = unit;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < p.stages && fill_row < p.N; ++i, fill_row += p.units) ring.refill(src, fill_row);
+  TeamSum<1, CL> sum{slots, bars.team, &abort_flag};
+  const float inv_width = 1.0f / static_cast<float>(p.width);
+  float4 wpre[VPT], wpost[VPT], gate[VPT];
+  int gate_row = -1;                // which row of the gate is held
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = i * T + threadIdx.x;
+    wpre[i] = v < vecs ? load_weight(p.wpre, vec0 + v, p.width) : zero4();
+    wpost[i] = post && v < vecs ? load_weight(p.wpost, vec0 + v, p.width) : ones4();
+    gate[i] = ones4();
+  }
+  int row = unit, lost = 0;
+  for (; row < p.N; row += p.units) {
+    if (p.gate != nullptr && row / p.gate_rows != gate_row) {
+      gate_row = row / p.gate_rows;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = i * T + threadIdx.x;
+        if (v < vecs) gate[i] = load_weight(p.gate + static_cast<long long>(gate_row) * p.M, vec0 + v, p.width);
+      }
     }
-  } else {
-    TeamSum<1, CL> team{slots, bars.team, &abort_flag, warps};
-    const int T = warps * 32;
-    const float inv_width = 1.0f / static_cast<float>(p.width);
-    float4 wpre[VPT], wpost[VPT];
+    const uint32_t at = ring.take();
+    if (at == 0u) { lost = ROLE_NORM_ROW; break; }
+    float4 b[VPT], r[VPT];
+    float t[1] = {0.0f}, rb = 1.0f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = i * T + threadIdx.x;
-      wpre[i] = v < vecs ? load_weight(p.wpre, vec0 + v, p.width) : zero4();
-      wpost[i] = v < vecs && p.wpost ? load_weight(p.wpost, vec0 + v, p.width) : ones4();
+      b[i] = v < vecs ? clip4(lds4(at + v * 16), (vec0 + v) * 4, p.width) : zero4();
+      r[i] = v < vecs ? clip4(lds4(at + p.slab_bytes + v * 16), (vec0 + v) * 4, p.width) : zero4();
+      t[0] += square_sum(b[i]);
     }
-    uint32_t s = 0, ph = 0;
-    for (int row = unit; row < p.N; row += p.units) {
-      if (!mbar_wait(smem_u32(&bars.full[s]), ph, &abort_flag)) {
-        give_up(p, &abort_flag, ROLE_NORM_ROW, row);
-        break;
-      }
-      float4 b[VPT], r[VPT];
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = i * T + threadIdx.x;
-        const uint32_t at = ring + s * p.stage_bytes + v * 16;
-        b[i] = v < vecs ? clip4(lds4(at), (vec0 + v) * 4, p.width) : zero4();
-        r[i] = v < vecs ? clip4(lds4(at + p.slab_bytes), (vec0 + v) * 4, p.width) : zero4();
-      }
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&bars.empty[s]));     // the row is in registers
-      if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1u; }
-      float rb = 1.0f, t[1];
-      if (p.wpost != nullptr) {
-        t[0] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) t[0] += square_sum(b[i]);
-        team.post(t);
-        if (!team.wait(t)) { give_up(p, &abort_flag, ROLE_NORM_ROW, row); break; }
-        rb = 1.0f / sqrtf(fmaf(t[0], inv_width, p.eps));
-        if (p.rstd_post != nullptr && threadIdx.x == 0 && rank == 0) p.rstd_post[row] = rb;
-      }
-      const long long base = static_cast<long long>(row) * p.M + vec0 * 4;
-      const float* gate = p.gate == nullptr ? nullptr : p.gate + static_cast<long long>(row / p.gate_rows) * p.M;
-      t[0] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = i * T + threadIdx.x;
-        if (v < vecs) {
-          r[i] = new_residual(p, b[i], r[i], rb, wpost[i], gate, vec0 + v);
-          *reinterpret_cast<float4*>(p.Rout + base + v * 4) = r[i];
-          t[0] += square_sum(r[i]);
-        }
-      }
-      team.post(t);
-      if (!team.wait(t)) { give_up(p, &abort_flag, ROLE_NORM_ROW, row); break; }
-      const float rr = 1.0f / sqrtf(fmaf(t[0], inv_width, p.eps));
-      if (p.rstd_pre != nullptr && threadIdx.x == 0 && rank == 0) p.rstd_pre[row] = rr;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = i * T + threadIdx.x;
-        if (v < vecs) *reinterpret_cast<float4*>(p.Y + base + v * 4) = scaled(r[i], rr, wpre[i]);
+    if (post) {
+      if (!sum(t)) { lost = ROLE_NORM_SUM; break; }
+      rb = inv_root(fmaf(t[0], inv_width, p.eps));
+      if (threadIdx.x == 0) {
+        if (fill_row < p.N) { ring.refill(src, fill_row); fill_row += p.units; }
+        if (p.rstd_post != nullptr && rank == 0) p.rstd_post[row] = rb;
       }
     }
+    const long long base = static_cast<long long>(row) * p.M + vec0 * 4;
+    t[0] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = i * T + threadIdx.x;
+      r[i] = new_residual(p, b[i], r[i], rb, wpost[i], gate[i]);
+      if (v < vecs) *reinterpret_cast<float4*>(p.Rout + base + v * 4) = r[i];
+      t[0] += square_sum(r[i]);
+    }
+    if (!sum(t)) { lost = ROLE_NORM_SUM; break; }
+    const float rr = inv_root(fmaf(t[0], inv_width, p.eps));
+    if (threadIdx.x == 0) {
+      if (!post && fill_row < p.N) { ring.refill(src, fill_row); fill_row += p.units; }
+      if (p.rstd_pre != nullptr && rank == 0) p.rstd_pre[row] = rr;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = i * T + threadIdx.x;
+      if (v < vecs) *reinterpret_cast<float4*>(p.Y + base + v * 4) = scaled(r[i], rr, wpre[i]);
+    }
+  }
+  if (lost) {
+    give_up(p, &abort_flag, lost, row);
+    if (threadIdx.x == 0) ring.land();
   }
   __syncthreads();
   if (CL > 1) cluster_sync();
@@ -388,178 +404,140 @@ struct UnitRows {
   }
 };
 
-// Block: the working warps, then one producer warp; the ring holds deltaY, R', B and deltaR' of a row.  The sums of
-// row i + 1 are formed and posted before the outputs of row i are, so nobody stands at a barrier for a row's reduction.
+// The ring holds deltaY, R', B and deltaR' of a row.  What the outputs need of a row beside its sums are three values per
+// element, a = deltaR' + q / rms(R'), r^ / rms(R') and b^: they stay in registers over the reduction.
 template <int CL, bool POST, bool GATE>
-__global__ void __launch_bounds__(544) norm_delta_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(RING_THREADS) norm_delta_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ __align__(8) RingBars bars;
   __shared__ float slots[2][3][64];
   __shared__ volatile int abort_flag;
-  const int warps = (blockDim.x >> 5) - 1;
-  ring_setup<CL>(&bars, &abort_flag, warps);
+  ring_setup<CL, 3>(&bars, &abort_flag, slots);
   const int rank = CL > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int unit = blockIdx.x / CL;
   const int vec0 = rank * p.vecs, vecs = min(p.vecs, p.M / 4 - vec0);
-  const uint32_t ring = smem_u32(ring_smem);
-  if ((threadIdx.x >> 5) == warps) {
-    if ((threadIdx.x & 31) == 0) {
-      const float* const src[4] = {p.dY, p.Rout, p.B, p.dRout};
-      UnitRows rows(p, unit);
-      produce(p, &bars, &abort_flag, ring, src, vecs * 16, vec0 * 4, [&]() -> long long { return rows.next(); });
+  const int T = blockDim.x;
+  const float* const src[4] = {p.dY, p.Rout, p.B, p.dRout};
+  Ring<4> ring{p, &bars, &abort_flag, smem_u32(ring_smem), static_cast<uint32_t>(vecs * 16), vec0 * 4};
+  UnitRows fill_rows(p, unit);
+  if (threadIdx.x == 0)
+    for (int i = 0, row; i < p.stages && (row = fill_rows.next()) >= 0; ++i) ring.refill(src, row);
+  // the column sums' blocks may take their places as this grid's blocks leave (they wait for its end before they read)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  TeamSum<3, CL> sum{slots, bars.team, &abort_flag};
+  const float inv_width = 1.0f / static_cast<float>(p.width);
+  const bool has_dr = p.dRout != nullptr;
+  float4 wpre[VPT], wpost[VPT], gate[VPT], dwpre[VPT], dwpost[VPT], dgate[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = i * T + threadIdx.x;
+    wpre[i] = v < vecs ? load_weight(p.wpre, vec0 + v, p.width) : zero4();
+    wpost[i] = POST && v < vecs ? load_weight(p.wpost, vec0 + v, p.width) : ones4();
+    gate[i] = ones4();
+    dwpre[i] = dwpost[i] = dgate[i] = zero4();
+  }
+  UnitRows rows(p, unit);
+  int row = rows.next(), group = -1, lost = 0;
+  float rb = POST && row >= 0 ? __ldg(p.rstd_post + row) : 1.0f, rr = row >= 0 ? __ldg(p.rstd_pre + row) : 0.0f;
+  while (row >= 0) {
+    if (GATE && rows.g != group) {
+      group = rows.g;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = i * T + threadIdx.x;
+        if (v < vecs) gate[i] = load_weight(p.gate + static_cast<long long>(group) * p.M, vec0 + v, p.width);
+      }
     }
-  } else {
-    TeamSum<3, CL> team{slots, bars.team, &abort_flag, warps};
-    const int T = warps * 32;
-    const float inv_width = 1.0f / static_cast<float>(p.width);
-    const bool has_dr = p.dRout != nullptr;
-    float4 wpre[VPT], wpost[VPT], dwpre[VPT], dwpost[VPT], dgate[VPT];
+    const int next_row = rows.next();
+    float next_rb = 1.0f, next_rr = 0.0f;      // a row ahead
+    if (next_row >= 0) {
+      if (POST) next_rb = __ldg(p.rstd_post + next_row);
+      next_rr = __ldg(p.rstd_pre + next_row);
+    }
+    const uint32_t at0 = ring.take();
+    if (at0 == 0u) { lost = ROLE_NORM_ROW; break; }
+    float4 a[VPT], c[VPT], b[VPT];
+    float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = i * T + threadIdx.x;
-      wpre[i] = v < vecs ? load_weight(p.wpre, vec0 + v, p.width) : zero4();
-      wpost[i] = POST && v < vecs ? load_weight(p.wpost, vec0 + v, p.width) : ones4();
-      dwpre[i] = dwpost[i] = dgate[i] = zero4();
-    }
-    struct Row { int row, g; float rb, rr; };
-    UnitRows rows(p, unit);
-    auto fetch = [&]() -> Row {       // the next row's index and its two factors, which are needed a row later
-      Row x;
-      x.row = rows.next();
-      x.g = rows.g;
-      x.rb = 1.0f; x.rr = 0.0f;
-      if (x.row >= 0) {
-        if (POST) x.rb = __ldg(p.rstd_post + x.row);
-        x.rr = __ldg(p.rstd_pre + x.row);
-      }
-      return x;
-    };
-    auto gate_at = [&](int g, int v) { return load_weight(p.gate + static_cast<long long>(g) * p.M, vec0 + v, p.width); };
-    // q r^, e (deltaR' + q / rms), e r^ / rms summed over the row; also deltaW_pre
-    auto sums_of = [&](const Row& x, uint32_t stage, float (&s)[3]) {
-      s[0] = s[1] = s[2] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = i * T + threadIdx.x;
-        if (v < vecs) {
-          const uint32_t at = ring + stage * p.stage_bytes + v * 16;
-          const int col = (vec0 + v) * 4;
-          const float4 dy = clip4(lds4(at), col, p.width);
-          const float4 ro = clip4(lds4(at + p.slab_bytes), col, p.width);
-          float4 b = zero4(), dr = zero4(), gt = ones4();
+      a[i] = c[i] = b[i] = zero4();
+      if (v < vecs) {
+        const uint32_t at = at0 + v * 16;
+        const int col = (vec0 + v) * 4;
+        const float4 dy = clip4(lds4(at), col, p.width);
+        const float4 ro = clip4(lds4(at + p.slab_bytes), col, p.width);
+        b[i] = clip4(lds4(at + 2 * p.slab_bytes), col, p.width);
+        if (has_dr) a[i] = clip4(lds4(at + 3 * p.slab_bytes), col, p.width);
+        auto one = [&](float dyv, float rv, float& av, float& cv, float& bv, float g, float w, float wo, float& dw) {
+          const float r = rv * rr, q = dyv * w;
+          if (POST) bv *= rb;
+          cv = r * rr;
+          av = fmaf(rr, q, av);
+          dw = fmaf(dyv, r, dw);
+          s[0] = fmaf(q, r, s[0]);
           if (POST) {
-            b = clip4(lds4(at + 2 * p.slab_bytes), col, p.width);
-            if (has_dr) dr = clip4(lds4(at + 3 * p.slab_bytes), col, p.width);
-            if (GATE) gt = gate_at(x.g, v);
+            const float e = p.scale * g * wo * bv;
+            s[1] = fmaf(e, av, s[1]);
+            s[2] = fmaf(e, cv, s[2]);
           }
-          auto one = [&](float dyv, float rv, float bv, float drv, float g, float w, float wo, float& dw) {
-            const float r = rv * x.rr, q = dyv * w;
-            dw = fmaf(dyv, r, dw);
-            s[0] = fmaf(q, r, s[0]);
-            if (POST) {
-              const float e = p.scale * g * wo * (bv * x.rb);
-              s[1] = fmaf(e, fmaf(x.rr, q, drv), s[1]);
-              s[2] = fmaf(e * x.rr, r, s[2]);
-            }
-          };
-          one(dy.x, ro.x, b.x, dr.x, gt.x, wpre[i].x, wpost[i].x, dwpre[i].x);
-          one(dy.y, ro.y, b.y, dr.y, gt.y, wpre[i].y, wpost[i].y, dwpre[i].y);
-          one(dy.z, ro.z, b.z, dr.z, gt.z, wpre[i].z, wpost[i].z, dwpre[i].z);
-          one(dy.w, ro.w, b.w, dr.w, gt.w, wpre[i].w, wpost[i].w, dwpre[i].w);
-        }
-      }
-    };
-    // deltaR, deltaB of the row; deltaW_post and deltaGate
-    auto outputs_of = [&](const Row& x, uint32_t stage, float c1, float c2) {
-      const long long base = static_cast<long long>(x.row) * p.M + vec0 * 4;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = i * T + threadIdx.x;
-        if (v < vecs) {
-          const uint32_t at = ring + stage * p.stage_bytes + v * 16;
-          const int col = (vec0 + v) * 4;
-          const float4 dy = clip4(lds4(at), col, p.width);
-          const float4 ro = clip4(lds4(at + p.slab_bytes), col, p.width);
-          const float4 b = POST || GATE ? clip4(lds4(at + 2 * p.slab_bytes), col, p.width) : zero4();
-          const float4 dr = has_dr ? clip4(lds4(at + 3 * p.slab_bytes), col, p.width) : zero4();
-          const float4 gt = GATE ? gate_at(x.g, v) : ones4();
-          float4 odr, odb;
-          auto one = [&](float dyv, float rv, float bv, float drv, float g, float w, float wo, float& o_dr, float& o_db,
-                         float& dpost, float& dgt) {
-            const float bh = POST ? bv * x.rb : bv;
-            const float dT = fmaf(x.rr, fmaf(-(rv * x.rr), c1, dyv * w), drv);
-            const float dP = p.scale * g * dT;
-            o_dr = p.res_scale * dT;
-            if (POST) {
-              o_db = x.rb * fmaf(-bh, c2, dP * wo);
-              dpost = fmaf(dP, bh, dpost);
-            } else {
-              o_db = dP;
-            }
-            if (GATE) dgt = fmaf(p.scale * bh * wo, dT, dgt);
-          };
-          one(dy.x, ro.x, b.x, dr.x, gt.x, wpre[i].x, wpost[i].x, odr.x, odb.x, dwpost[i].x, dgate[i].x);
-          one(dy.y, ro.y, b.y, dr.y, gt.y, wpre[i].y, wpost[i].y, odr.y, odb.y, dwpost[i].y, dgate[i].y);
-          one(dy.z, ro.z, b.z, dr.z, gt.z, wpre[i].z, wpost[i].z, odr.z, odb.z, dwpost[i].z, dgate[i].z);
-          one(dy.w, ro.w, b.w, dr.w, gt.w, wpre[i].w, wpost[i].w, odr.w, odb.w, dwpost[i].w, dgate[i].w);
-          *reinterpret_cast<float4*>(p.dR + base + v * 4) = odr;     // padding columns: every operand was cleared
-          *reinterpret_cast<float4*>(p.dB + base + v * 4) = odb;
-        }
-      }
-    };
-    uint32_t s = 0, ph = 0;           // ring position of the row whose sums come next
-    auto advance = [&]() { if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1u; } };
-    Row cur = fetch(), nxt = fetch();
-    float t[3], c[3];
-    uint32_t stage = 0;
-    bool alive = cur.row >= 0;
-    if (alive) {
-      alive = mbar_wait(smem_u32(&bars.full[s]), ph, &abort_flag);
-      if (alive) {
-        sums_of(cur, s, t);
-        team.post(t);
-        stage = s;
-        advance();
-        alive = team.wait(c);
+        };
+        one(dy.x, ro.x, a[i].x, c[i].x, b[i].x, gate[i].x, wpre[i].x, wpost[i].x, dwpre[i].x);
+        one(dy.y, ro.y, a[i].y, c[i].y, b[i].y, gate[i].y, wpre[i].y, wpost[i].y, dwpre[i].y);
+        one(dy.z, ro.z, a[i].z, c[i].z, b[i].z, gate[i].z, wpre[i].z, wpost[i].z, dwpre[i].z);
+        one(dy.w, ro.w, a[i].w, c[i].w, b[i].w, gate[i].w, wpre[i].w, wpost[i].w, dwpre[i].w);
       }
     }
-    while (alive && cur.row >= 0) {
-      const uint32_t next_stage = s;
-      const Row after = nxt.row >= 0 ? fetch() : nxt;
-      if (nxt.row >= 0) {
-        alive = mbar_wait(smem_u32(&bars.full[s]), ph, &abort_flag);
-        if (!alive) break;
-        sums_of(nxt, s, t);
-        team.post(t);
-        advance();
-      }
-      const float c1 = c[0] * inv_width;
-      outputs_of(cur, stage, c1, fmaf(-c1, c[2], c[1]) * inv_width);
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&bars.empty[stage]));
-      if (GATE && p.gate_direct && (nxt.row < 0 || nxt.g != cur.g)) {     // the group's rows are done
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-          const int v = i * T + threadIdx.x;
-          if (v < vecs) *reinterpret_cast<float4*>(p.dgate + static_cast<long long>(cur.g) * p.M + (vec0 + v) * 4) = dgate[i];
-          dgate[i] = zero4();
-        }
-      }
-      if (nxt.row >= 0) alive = team.wait(c);
-      cur = nxt;
-      nxt = after;
-      stage = next_stage;
+    if (!sum(s)) { lost = ROLE_NORM_SUM; break; }
+    if (threadIdx.x == 0) {
+      const int more = fill_rows.next();
+      if (more >= 0) ring.refill(src, more);
     }
-    if (!alive && cur.row >= 0 && (threadIdx.x & 31) == 0) give_up(p, &abort_flag, ROLE_NORM_ROW, cur.row);
+    const float c1 = s[0] * inv_width, c2 = fmaf(-c1, s[2], s[1]) * inv_width;
+    const long long base = static_cast<long long>(row) * p.M + vec0 * 4;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = i * T + threadIdx.x;
       if (v < vecs) {
-        const long long at = static_cast<long long>(unit) * p.M + (vec0 + v) * 4;
-        *reinterpret_cast<float4*>(p.part_pre + at) = dwpre[i];
-        if (POST) *reinterpret_cast<float4*>(p.part_post + at) = dwpost[i];
-        if (GATE && !p.gate_direct) *reinterpret_cast<float4*>(p.part_gate + at) = dgate[i];
+        float4 odr, odb;
+        auto one = [&](float av, float cv, float bv, float g, float wo, float& o_dr, float& o_db, float& dpost, float& dgt) {
+          const float dT = fmaf(-cv, c1, av);
+          const float dP = p.scale * g * dT;
+          o_dr = p.res_scale * dT;
+          o_db = POST ? rb * fmaf(-bv, c2, dP * wo) : dP;
+          if (POST) dpost = fmaf(dP, bv, dpost);
+          if (GATE) dgt = fmaf(p.scale * bv * wo, dT, dgt);
+        };
+        one(a[i].x, c[i].x, b[i].x, gate[i].x, wpost[i].x, odr.x, odb.x, dwpost[i].x, dgate[i].x);
+        one(a[i].y, c[i].y, b[i].y, gate[i].y, wpost[i].y, odr.y, odb.y, dwpost[i].y, dgate[i].y);
+        one(a[i].z, c[i].z, b[i].z, gate[i].z, wpost[i].z, odr.z, odb.z, dwpost[i].z, dgate[i].z);
+        one(a[i].w, c[i].w, b[i].w, gate[i].w, wpost[i].w, odr.w, odb.w, dwpost[i].w, dgate[i].w);
+        *reinterpret_cast<float4*>(p.dR + base + v * 4) = odr;     // padding columns: every operand was cleared
+        *reinterpret_cast<float4*>(p.dB + base + v * 4) = odb;
       }
+    }
+    if (GATE && p.gate_direct && (next_row < 0 || rows.g != group)) {     // the group's rows are done
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = i * T + threadIdx.x;
+        if (v < vecs) *reinterpret_cast<float4*>(p.dgate + static_cast<long long>(group) * p.M + (vec0 + v) * 4) = dgate[i];
+        dgate[i] = zero4();
+      }
+    }
+    row = next_row; rb = next_rb; rr = next_rr;
+  }
+  if (lost) {
+    give_up(p, &abort_flag, lost, row);
+    if (threadIdx.x == 0) ring.land();
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = i * T + threadIdx.x;
+    if (v < vecs) {
+      const long long at = static_cast<long long>(unit) * p.M + (vec0 + v) * 4;
+      *reinterpret_cast<float4*>(p.part_pre + at) = dwpre[i];
+      if (POST) *reinterpret_cast<float4*>(p.part_post + at) = dwpost[i];
+      if (GATE && !p.gate_direct) *reinterpret_cast<float4*>(p.part_gate + at) = dgate[i];
     }
   }
   __syncthreads();
@@ -583,6 +561,7 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
   const int v = blockIdx.x * 8 + c;
   const int rows = p.rows[z];
   float4 s = zero4();
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // the partial rows are complete
   if (v < p.M / 4) {
     const float4* src = reinterpret_cast<const float4*>(in) + static_cast<long long>(blockIdx.y) * rows * (p.M / 4) + v;
 #pragma unroll 4
@@ -605,9 +584,10 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
 // ------------------------------------------------------------------ host
 // How a row of M floats is laid on a persistent kernel: blocks per row, vectors per block, working threads, and a ring of
 // rows of `arrays` parts that leaves room for the blocks an SM takes.
+constexpr int FORWARD_REGS = 64, DELTA_REGS = 128;      // what the kernels are compiled to at their launch bounds
 struct Shape { int cl, vecs, threads, stages, stage_bytes, slab_bytes, per_sm; };
 
-Shape ring_shape(int M, int arrays) {
+Shape ring_shape(int M, int arrays, int regs) {
   Shape s{};
   const int all = M / 4;
   s.cl = all <= 1024 ? 1 : (all <= 2048 ? 2 : 4);
@@ -615,8 +595,8 @@ Shape ring_shape(int M, int arrays) {
   s.threads = ((s.vecs + VPT - 1) / VPT + 31) / 32 * 32;
   s.slab_bytes = s.vecs * 16;
   s.stage_bytes = (s.slab_bytes * arrays + 127) / 128 * 128;
-  // blocks per SM: by shared memory at three rows each, by registers (at most 112 per thread: 544 threads fit once)
-  const int by_smem = 220 * 1024 / (3 * s.stage_bytes + 2048), by_regs = 585 / (s.threads + 32);
+  // blocks per SM: by shared memory at three rows each, by the registers per thread
+  const int by_smem = 220 * 1024 / (3 * s.stage_bytes + 2048), by_regs = 65536 / (regs * s.threads);
   s.per_sm = by_smem < by_regs ? by_smem : by_regs;
   if (s.per_sm < 1) s.per_sm = 1;
   s.stages = (220 * 1024 / s.per_sm - 2048) / s.stage_bytes;
@@ -634,7 +614,7 @@ int cluster_count() {
   if (n > 0) return n;
   cudaLaunchConfig_t q = {};
   q.gridDim = dim3(static_cast<unsigned>(device_sm_count() / CL * CL), 1, 1);
-  q.blockDim = dim3(544, 1, 1);
+  q.blockDim = dim3(RING_THREADS, 1, 1);
   q.dynamicSmemBytes = 210 * 1024;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -675,7 +655,7 @@ cudaError_t launch_ring(const Shape& s, NormParams p, cudaStream_t st) {
   p.vecs = s.vecs; p.stages = s.stages; p.stage_bytes = s.stage_bytes; p.slab_bytes = s.slab_bytes;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.units) * s.cl, 1, 1);
-  cfg.blockDim = dim3(s.threads + 32, 1, 1);
+  cfg.blockDim = dim3(s.threads, 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(s.stages) * s.stage_bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -763,7 +743,7 @@ int cu32_normResidual(int64_t stream, const float* B, const float* R, const floa
     else norm_forward_kernel<4><<<N, threads, 0, st>>>(p);
     return static_cast<int>(cudaPeekAtLastError());
   }
-  const Shape s = ring_shape(M, 2);
+  const Shape s = ring_shape(M, 2, FORWARD_REGS);
   p.units = ring_units(s);
   if (p.units > N) p.units = N;
   if (s.cl == 1) return static_cast<int>(launch_ring<norm_forward_ring_kernel<1>>(s, p, st));
@@ -773,7 +753,7 @@ int cu32_normResidual(int64_t stream, const float* B, const float* R, const floa
 
 long long cu32_normResidual_work(int N, int M, int gate_rows) {
   if (check_rows(N, M, M, gate_rows)) return 0;
-  return work_floats_of(plan_rows(N, gate_rows, ring_units(ring_shape(M, 4))), M);
+  return work_floats_of(plan_rows(N, gate_rows, ring_units(ring_shape(M, 4, DELTA_REGS))), M);
 }
 
 int cu32_normResidual_delta(int64_t stream, const float* dRout, const float* dY, const float* B, const float* Rout,
@@ -785,7 +765,7 @@ int cu32_normResidual_delta(int64_t stream, const float* dRout, const float* dY,
   if (int rc = check_rows(N, M, width, gate_rows)) return rc;
   if (gate && gate_rows == 0) return CU32_E_DIM;
   if (!all_aligned16(dRout, dY, B, Rout, gate, wpost, wpre, dR, dB, dgate, dwpost, dwpre, work)) return CU32_E_ALIGN;
-  const Shape s = ring_shape(M, 4);
+  const Shape s = ring_shape(M, 4, DELTA_REGS);
   int want = ring_units(s);
   const long long room = work_floats / (3LL * M);
   if (room < 1) return CU32_E_SCRATCH;
@@ -815,8 +795,16 @@ int cu32_normResidual_delta(int64_t stream, const float* dRout, const float* dY,
   const bool gate_sum = gate && !r.direct;
   if (gate_sum) { c.in[2] = p.part_gate; c.out[2] = dgate; c.rows[2] = r.chunks; }
   const dim3 grid(static_cast<unsigned>((M / 4 + 7) / 8), gate_sum ? static_cast<unsigned>(r.groups) : 1u, gate_sum ? 3u : 2u);
-  column_sum_kernel<<<grid, 256, 0, st>>>(c);
-  return static_cast<int>(cudaPeekAtLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, column_sum_kernel, c));
 }
 
 }  // extern "C"
