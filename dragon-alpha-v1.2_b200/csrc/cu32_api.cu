@@ -121,13 +121,17 @@ bool load_driver_entry_points() {
 int make_map3(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint64_t d2,
                      uint64_t pitch1_floats, uint64_t pitch2_floats, uint32_t b0, uint32_t b1,
                      bool mn_major) {
+  return make_map3_as(m, base, d0, d1, d2, pitch1_floats, pitch2_floats, b0, b1,
+                      mn_major ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int make_map3_as(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t pitch1_floats,
+                 uint64_t pitch2_floats, uint32_t b0, uint32_t b1, CUtensorMapSwizzle swizzle) {
   cuuint64_t dims[3] = {d0, d1, d2};
   cuuint64_t strides[2] = {pitch1_floats * 4, pitch2_floats * 4};
   cuuint32_t box[3] = {b0, b1, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = g_encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims,
-                              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              mn_major ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+                              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? CU32_OK : CU32_E_TENSORMAP;
 }

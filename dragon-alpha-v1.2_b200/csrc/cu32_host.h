@@ -44,6 +44,8 @@ bool load_driver_entry_points();
 // 3-D FP32 map (inner, outer, batch) with zero fill; see cu32_api.cu for the swizzles.
 int make_map3(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t pitch1_floats,
               uint64_t pitch2_floats, uint32_t b0, uint32_t b1, bool mn_major);
+int make_map3_as(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t pitch1_floats,
+                 uint64_t pitch2_floats, uint32_t b0, uint32_t b1, CUtensorMapSwizzle swizzle);
 // k-blocks per in-TMEM chunk of the FP32-accurate mode (the "kc" tuning key).
 int tuned_kc();
 // The "tile" tuning key: a forced tile configuration, or -1.

@@ -9,7 +9,6 @@
 // and the two products of deltaX in one accumulation.  6 N D F flop forward and 12 N D F backward at the
 // FP32-accurate rate bound it.
 // Few rows: every weight is read once for all rows, so the time is that of reading 3 D F floats; rows_kernel below.
-#include <cooperative_groups.h>
 #include <atomic>
 
 #include "cu32_host.h"
@@ -17,203 +16,423 @@
 namespace dragon {
 namespace {
 
-namespace cg = cooperative_groups;
+using namespace ptx;
 
 // ------------------------------------------------------------------ few rows
 struct RowsParams {
-  const float* X;             // [N, K]
-  const float* W[2];          // [K, M]; the second only for the gated form
+  CUtensorMap tmW[2];         // [K, M] weights, boxes of KT rows x CPW columns; the second only for the gated form
+  CUtensorMap tmX;            // [N, K] operand, boxes of NR rows x KT columns
   float* out;                 // [N, M]
   float* G;                   // gated form: pre-activations, or null
   float* U;
-  int N, M, K, act;
-  int kc;                     // rows of K staged at a time
+  int N, M, act;
+  int ktiles, items, clusters, stages;
+  int early;                  // the grid may start before the one that writes X has ended
+  int* status;
 };
 
-__device__ __forceinline__ float4 ldg_stream(const float* p) {
+constexpr int ROWS_WARPS = 8, ROWS_WORKERS = ROWS_WARPS * 32, ROWS_THREADS = ROWS_WORKERS + 32;
+constexpr int ROWS_MAX_STAGES = 12;
+constexpr int ROLE_ROWS_LOAD = 10, ROLE_ROWS_TILE = 11, ROLE_ROWS_SUM = 12;
+
+__device__ __forceinline__ float4 lds_v4(uint32_t addr) {
   float4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void sts_v4(uint32_t addr, float4 v) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+// Pairs of floats in one 64-bit register: fma.rn.f32x2 does both products in one issue, at twice the scalar rate.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ void lds_pairs(uint32_t addr, f32x2& a, f32x2& b) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr));
+}
+__device__ __forceinline__ f32x2 both(float x) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void fma_pair(f32x2& acc, f32x2 a, f32x2 b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b)); }
+__device__ __forceinline__ float2 unpack(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ float2 lds_v2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+  return v;
+}
+// 16 bytes to a block of the cluster, counted by that block's barrier
+__device__ __forceinline__ void st_async_v4(uint32_t addr, float4 v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(addr), "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)),
+                 "r"(__float_as_uint(v.w)), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(ROWS_WORKERS) : "memory"); }
 
-constexpr int ROWS_THREADS = 256, ROWS_WARPS = ROWS_THREADS / 32;
+// Shared memory of a block: [ring of tiles][sums of the warps, four rows at a time][inbox, two items]
+template <int NR, int MATS, int CPW, int S>
+struct RowsCfg {
+  static constexpr int KT = 4096 / CPW;                                 // rows of the weights per tile: 16 KB a matrix
+  static constexpr int W_BYTES = KT * CPW * 4, X_BYTES = NR * KT * 4;
+  static constexpr int TILE_BYTES = MATS * W_BYTES + (X_BYTES + 127) / 128 * 128;
+  static constexpr int GROUP = NR < 4 ? NR : 4;                         // rows reduced at a time
+  static constexpr int RED_BYTES = ROWS_WARPS * GROUP * MATS * CPW * 4;
+  static constexpr int BOX_BYTES = NR * MATS * CPW * 4;                 // an item's sums from all blocks of the cluster
+  static constexpr int FIXED = RED_BYTES + 2 * BOX_BYTES + 128;
+  static constexpr int STAGES_FIT = (224 * 1024 - FIXED) / TILE_BYTES;
+  static constexpr int STAGES = STAGES_FIT < ROWS_MAX_STAGES ? STAGES_FIT : ROWS_MAX_STAGES;
+  static constexpr int SMEM = FIXED + STAGES * TILE_BYTES;
+  static_assert(STAGES >= 3, "ring");
+};
 
 // out[n, :] = X[n, :] W  (MATS = 1)  or  act(X[n, :] W0) * (X[n, :] W1)  (MATS = 2)  for N <= NR rows.
-// A cluster owns CPW columns and its CTAs a slice of K each; inside a CTA the warps take every eighth (group of) row(s)
-// of the weights, 16 bytes per lane.  X's slice sits in shared memory as [k][NR], so one broadcast read serves four rows.
-// The partial sums of lanes, warps and CTAs are added in a fixed order: results do not vary from run to run.
-template <int NR, int MATS, int CPW>
-__global__ void __launch_bounds__(ROWS_THREADS) rows_kernel(const __grid_constant__ RowsParams p) {
-  extern __shared__ float4 rows_smem4[];
-  float* sm = reinterpret_cast<float*>(rows_smem4);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int S = static_cast<int>(cluster.num_blocks());
-  const int rank = static_cast<int>(cluster.block_rank());
-  constexpr int LPR = CPW / 4, KPW = 32 / LPR, STEP = ROWS_WARPS * KPW;
-  constexpr int UN = MATS == 2 ? 4 : 8;
+// The weights are read once for all rows: the time is theirs.  A producer warp keeps a ring of weight tiles (KT rows x CPW
+// columns, with the KT columns of X that meet them) full by TMA whatever the workers do; the persistent cluster takes
+// blocks of CPW columns in turn, its S blocks a slice of K each.  A worker holds 4 columns x NR rows of sums; the sums of
+// lanes, warps and blocks are added in a fixed order, each block of the cluster finishing CPW / S columns.
+// (Measured with plain loads into registers instead of the ring, one launch over all column blocks: 184 us for 8 rows of
+// a 4096 / 10924 layer, 537 MB.)
+template <int NR, int MATS, int CPW, int S>
+__global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_constant__ RowsParams p) {
+  using Cfg = RowsCfg<NR, MATS, CPW, S>;
+  extern __shared__ __align__(128) uint8_t rows_smem[];
+  __shared__ __align__(8) uint64_t bar_full[ROWS_MAX_STAGES], bar_empty[ROWS_MAX_STAGES], bar_box[2];
+  __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col0 = (blockIdx.x / S) * CPW;
-  const int col = col0 + (lane % LPR) * 4;
-  const bool col_ok = col < p.M;    // M is a multiple of 4
-  const int k0 = static_cast<int>(static_cast<long long>(rank) * p.K / S);
-  const int k1 = static_cast<int>(static_cast<long long>(rank + 1) * p.K / S);
-  float acc[NR][MATS][4];
-#pragma unroll
-  for (int n = 0; n < NR; ++n)
-#pragma unroll
-    for (int m = 0; m < MATS; ++m)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[n][m][c] = 0.0f;
-
-  for (int kb = k0; kb < k1; kb += p.kc) {
-    const int ke = min(kb + p.kc, k1);
-    __syncthreads();                      // the previous slice has been read
-    for (int i = threadIdx.x; i < (ke - kb) * NR; i += ROWS_THREADS) {
-      const int n = i / (ke - kb), k = i - n * (ke - kb);
-      sm[k * NR + n] = n < p.N ? p.X[static_cast<long long>(n) * p.K + kb + k] : 0.0f;
+  const uint32_t rank = S > 1 ? cluster_ctarank() : 0u;
+  const uint32_t ring = (smem_u32(rows_smem) + 127u) & ~127u;
+  const uint32_t red = ring + Cfg::STAGES * Cfg::TILE_BYTES, box = red + Cfg::RED_BYTES;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < ROWS_MAX_STAGES; ++i) {
+      mbar_init(smem_u32(&bar_full[i]), 1);
+      mbar_init(smem_u32(&bar_empty[i]), ROWS_WARPS);
     }
-    __syncthreads();
-    for (int k = kb + warp * KPW + lane / LPR; k < ke; k += STEP * UN) {
-      float4 w[UN][MATS];
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bar_box[i]), 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (S > 1) cluster_sync();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int first_item = blockIdx.x / S;
+  const int t0 = static_cast<int>(rank) * p.ktiles / S, t1 = (static_cast<int>(rank) + 1) * p.ktiles / S;
+  auto give_up = [&](int role, int it) {
+    abort_flag = 1;
+    atomicCAS(p.status, 0, (role << 24) | (it & 0xFFFF));
+  };
+
+  if (warp == ROWS_WARPS) {
+    if (lane == 0) {
+      // Weight tiles may be on their way before X exists: only X's loads wait for the grid that writes it.
+      auto load_w = [&](uint32_t st, int item, int t) {
+        const uint32_t bar = smem_u32(&bar_full[st]), dst = ring + st * Cfg::TILE_BYTES;
+        mbar_arrive_expect_tx(bar, MATS * Cfg::W_BYTES + Cfg::X_BYTES);
 #pragma unroll
-      for (int u = 0; u < UN; ++u)
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-          const int kk = k + u * STEP;
-          w[u][m] = (kk < ke && col_ok) ? ldg_stream(p.W[m] + static_cast<long long>(kk) * p.M + col)
-                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int m = 0; m < MATS; ++m) tma_load_3d(dst + m * Cfg::W_BYTES, &p.tmW[m], bar, item * CPW, t * Cfg::KT, 0, 0ull);
+      };
+      auto load_x = [&](uint32_t st, int t) {
+        tma_load_3d(ring + st * Cfg::TILE_BYTES + MATS * Cfg::W_BYTES, &p.tmX, smem_u32(&bar_full[st]), t * Cfg::KT, 0, 0, 0ull);
+      };
+      uint32_t st = 0, ph = 0, it = 0;
+      int early_x[ROWS_MAX_STAGES];
+      int held = 0;                        // tiles whose X has not been asked for yet
+      bool started = p.early == 0, alive = true;
+      for (int item = first_item; alive && item < p.items; item += p.clusters) {
+        for (int t = t0; t < t1; ++t, ++it) {
+          if (!started && held == Cfg::STAGES) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int i = 0; i < held; ++i) load_x(i, early_x[i]);
+            started = true;
+          }
+          if (!mbar_wait(smem_u32(&bar_empty[st]), ph ^ 1u, &abort_flag)) {
+            give_up(ROLE_ROWS_LOAD, it);
+            alive = false;
+            break;
+          }
+          load_w(st, item, t);
+          if (started) load_x(st, t);
+          else early_x[held++] = t;
+          if (++st == Cfg::STAGES) { st = 0; ph ^= 1u; }
         }
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int kk = min(k + u * STEP, ke - 1);
-        const float* x = sm + (kk - kb) * NR;
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          const float xv = x[n];
-#pragma unroll
-          for (int m = 0; m < MATS; ++m) {
-            acc[n][m][0] = fmaf(xv, w[u][m].x, acc[n][m][0]);
-            acc[n][m][1] = fmaf(xv, w[u][m].y, acc[n][m][1]);
-            acc[n][m][2] = fmaf(xv, w[u][m].z, acc[n][m][2]);
-            acc[n][m][3] = fmaf(xv, w[u][m].w, acc[n][m][3]);
+      }
+      if (!started) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (int i = 0; i < held; ++i) load_x(i, early_x[i]);
+      }
+      if (abort_flag) {                    // copies in flight land before the block may leave
+        const uint32_t n = it < static_cast<uint32_t>(Cfg::STAGES) ? it : static_cast<uint32_t>(Cfg::STAGES);
+        for (uint32_t i = it - n; i < it; ++i) {
+          const long long c0 = clock64();
+          while (!mbar_try_wait(smem_u32(&bar_full[i % Cfg::STAGES]), (i / Cfg::STAGES) & 1u) && clock64() - c0 < 20000000LL) {
           }
         }
       }
     }
-  }
-  // lanes of a warp that hold the same columns
+  } else {
+    constexpr int LPR = CPW / 4;           // lanes per row of the tile
+    constexpr int RPL = 4;                 // rows of the tile per lane
+    const int k_in = (warp * (32 / LPR) + lane / LPR) * RPL, c_in = (lane % LPR) * 4;
+    uint32_t st = 0, ph = 0, done = 0;
+    bool alive = true;
+    for (int item = first_item; alive && item < p.items; item += p.clusters, ++done) {
+      f32x2 acc2[NR][MATS][2];
 #pragma unroll
-  for (int o = LPR; o < 32; o <<= 1)
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
+        for (int m = 0; m < MATS; ++m) acc2[n][m][0] = acc2[n][m][1] = 0ull;
+      // A lane's four rows of a tile go in two parts of two; the loads of a part are under way during the products of the
+      // part before it, across tiles too, and a tile is given back as soon as its second part has been read.
+      constexpr int JB = RPL / 2;
+      struct Part { f32x2 w[JB][MATS][2]; float2 x[NR]; };
+      auto load = [&](Part& q, uint32_t tile, int j0) {
 #pragma unroll
-      for (int m = 0; m < MATS; ++m)
+        for (int j = 0; j < JB; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[n][m][c] += __shfl_xor_sync(0xffffffffu, acc[n][m][c], o);
-  __syncthreads();
-  constexpr int PER = NR * MATS * CPW;    // sums of a CTA: [n][m][column]
-  if (lane < LPR) {
+          for (int m = 0; m < MATS; ++m)
+            lds_pairs(tile + m * Cfg::W_BYTES + ((k_in + j0 + j) * CPW + c_in) * 4, q.w[j][m][0], q.w[j][m][1]);
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
+        for (int n = 0; n < NR; ++n) q.x[n] = lds_v2(tile + MATS * Cfg::W_BYTES + (n * Cfg::KT + k_in + j0) * 4);
+      };
+      auto multiply = [&](const Part& q) {
 #pragma unroll
-      for (int m = 0; m < MATS; ++m)
-        *reinterpret_cast<float4*>(sm + warp * PER + (n * MATS + m) * CPW + lane * 4) =
-            make_float4(acc[n][m][0], acc[n][m][1], acc[n][m][2], acc[n][m][3]);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < PER; i += ROWS_THREADS) {
-    float s = sm[i];
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int w = 1; w < ROWS_WARPS; ++w) s += sm[w * PER + i];
-    sm[i] = s;
-  }
-  cluster.sync();
-  // the CTAs of the cluster share the outputs: each adds the S partial sums of its part
-  for (int i = rank * ROWS_THREADS + threadIdx.x; i < NR * CPW; i += S * ROWS_THREADS) {
-    const int n = i / CPW, c = i - n * CPW;
-    if (n < p.N && col0 + c < p.M) {
-      float v[MATS];
+          for (int j = 0; j < JB; ++j) {
+            const f32x2 x = both(j == 0 ? q.x[n].x : q.x[n].y);
 #pragma unroll
-      for (int m = 0; m < MATS; ++m) {
-        float s = 0.0f;
-        for (int r = 0; r < S; ++r) s += cluster.map_shared_rank(sm, r)[(n * MATS + m) * CPW + c];
-        v[m] = s;
+            for (int m = 0; m < MATS; ++m) {
+              fma_pair(acc2[n][m][0], x, q.w[j][m][0]);
+              fma_pair(acc2[n][m][1], x, q.w[j][m][1]);
+            }
+          }
+      };
+      auto arrived = [&](int t) {
+        if (mbar_wait(smem_u32(&bar_full[st]), ph, &abort_flag)) return true;
+        if (lane == 0) give_up(ROLE_ROWS_TILE, t);
+        return false;
+      };
+      Part a, b;
+      alive = arrived(t0);
+      if (alive) load(a, ring + st * Cfg::TILE_BYTES, 0);
+      for (int t = t0; alive && t < t1; ++t) {
+        load(b, ring + st * Cfg::TILE_BYTES, JB);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_empty[st]));
+        if (++st == Cfg::STAGES) { st = 0; ph ^= 1u; }
+        multiply(a);
+        if (t + 1 < t1) {
+          alive = arrived(t + 1);
+          if (alive) load(a, ring + st * Cfg::TILE_BYTES, 0);
+        }
+        multiply(b);
       }
-      const long long at = static_cast<long long>(n) * p.M + col0 + c;
-      if (MATS == 2) {
-        if (p.G != nullptr) { p.G[at] = v[0]; p.U[at] = v[MATS - 1]; }
-        float pair[2] = {v[0], v[MATS - 1]};
-        gated_forward<1>(p.act, pair);
-        p.out[at] = pair[0];
-      } else {
-        p.out[at] = v[0];
+      if (!alive) break;
+      float acc[NR][MATS][4];
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+          const float2 lo = unpack(acc2[n][m][0]), hi = unpack(acc2[n][m][1]);
+          acc[n][m][0] = lo.x; acc[n][m][1] = lo.y; acc[n][m][2] = hi.x; acc[n][m][3] = hi.y;
+        }
+      // lanes of a warp that hold the same columns
+#pragma unroll
+      for (int o = LPR; o < 32; o <<= 1)
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[n][m][c] += __shfl_xor_sync(0xffffffffu, acc[n][m][c], o);
+      // Sums of the warps, four rows at a time; each goes to the inbox of the block that finishes its columns:
+      // inbox[item parity][from][n][m][CPW / S columns].  The place is free: whoever sends item i + 2 has received every
+      // block's item i + 1, which each sent after it had read item i.
+      constexpr int CV = CPW / 4, OV = CV / S;        // vectors per row of the item, and per owner
+      const uint32_t par = done & 1u, inbox = box + par * Cfg::BOX_BYTES;
+      if (threadIdx.x == 0) mbar_arrive_expect_tx(smem_u32(&bar_box[par]), Cfg::BOX_BYTES);
+#pragma unroll
+      for (int g = 0; g < NR; g += Cfg::GROUP) {
+        if (lane < LPR) {
+#pragma unroll
+          for (int n = 0; n < Cfg::GROUP; ++n)
+#pragma unroll
+            for (int m = 0; m < MATS; ++m)
+              sts_v4(red + (((warp * Cfg::GROUP + n) * MATS + m) * CV + lane) * 16,
+                     make_float4(acc[g + n][m][0], acc[g + n][m][1], acc[g + n][m][2], acc[g + n][m][3]));
+        }
+        workers_sync();
+        for (int e = threadIdx.x; e < Cfg::GROUP * MATS * CV; e += ROWS_WORKERS) {
+          float4 v = lds_v4(red + e * 16);
+#pragma unroll
+          for (int w = 1; w < ROWS_WARPS; ++w) {
+            const float4 u = lds_v4(red + (w * Cfg::GROUP * MATS * CV + e) * 16);
+            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+          }
+          const int nm = g * MATS + e / CV, c = e % CV;       // (n * MATS + m), vector of the row
+          const uint32_t owner = c / OV;
+          const uint32_t at = inbox + ((rank * NR * MATS + nm) * OV + c % OV) * 16;
+          const uint32_t bar = smem_u32(&bar_box[par]);
+          if (S == 1) st_async_v4(mapa(at, 0u), v, mapa(bar, 0u));
+          else st_async_v4(mapa(at, owner), v, mapa(bar, owner));
+        }
+        workers_sync();
       }
+      if (!mbar_wait(smem_u32(&bar_box[par]), (done >> 1) & 1u, &abort_flag)) {
+        if (lane == 0) give_up(ROLE_ROWS_SUM, item);
+        break;
+      }
+      for (int e = threadIdx.x; e < NR * OV; e += ROWS_WORKERS) {
+        const int n = e / OV, c = e % OV;
+        const int col = item * CPW + (static_cast<int>(rank) * OV + c) * 4;
+        float v[MATS * 4];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int r = 0; r < S; ++r) {
+            const float4 u = lds_v4(inbox + ((r * NR * MATS + n * MATS + m) * OV + c) * 16);
+            a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+          }
+          v[m * 4] = a.x; v[m * 4 + 1] = a.y; v[m * 4 + 2] = a.z; v[m * 4 + 3] = a.w;
+        }
+        if (n < p.N && col < p.M) {          // M is a multiple of 4
+          const long long at = static_cast<long long>(n) * p.M + col;
+          if constexpr (MATS == 2) {
+            if (p.G != nullptr) {
+              *reinterpret_cast<float4*>(p.G + at) = make_float4(v[0], v[1], v[2], v[3]);
+              *reinterpret_cast<float4*>(p.U + at) = make_float4(v[4], v[5], v[6], v[7]);
+            }
+            gated_forward<4>(p.act, v);
+          }
+          *reinterpret_cast<float4*>(p.out + at) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      workers_sync();                        // the inbox has been read before this block sends its next item
     }
   }
-  cluster.sync();     // nobody leaves while its sums are being read
+  __syncthreads();
+  if (S > 1) cluster_sync();                 // nobody leaves while a block may still send to it
 }
 
-template <int NR, int MATS, int CPW>
-int rows_launch_one(RowsParams p, int S, cudaStream_t st) {
-  constexpr int SLICE = 16384;            // floats of X staged at a time (64 KB)
-  p.kc = SLICE / NR;
-  const int klen = (p.K + S - 1) / S;
-  if (p.kc > klen) p.kc = klen;
-  constexpr int RED = ROWS_WARPS * NR * MATS * CPW;
-  const size_t smem = sizeof(float) * static_cast<size_t>(p.kc * NR > RED ? p.kc * NR : RED);
-  constexpr size_t MAX_SMEM = sizeof(float) * (SLICE > RED ? SLICE : RED);
-  auto kernel = rows_kernel<NR, MATS, CPW>;
-  static std::atomic<int> ready[64];      // per device: the shared-memory opt-in has been made
+// 2-D map without swizzle: rows of `inner` floats, boxes of b1 rows x b0 floats, zeros outside.
+int make_map_rows(CUtensorMap* m, const float* base, uint64_t inner, uint64_t rows, uint32_t b0, uint32_t b1) {
+  return make_map3_as(m, base, inner, rows, 1, inner, inner * rows, b0, b1, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+// Clusters of S blocks that run at the same time (asked once per device and kernel).
+template <int NR, int MATS, int CPW, int S>
+cudaError_t rows_clusters(int* count) {
+  using Cfg = RowsCfg<NR, MATS, CPW, S>;
+  auto kernel = rows_kernel<NR, MATS, CPW, S>;
+  static std::atomic<int> cache[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (!ready[dev & 63].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM));
-    if (e != cudaSuccess) return static_cast<int>(e);
-    ready[dev & 63].store(1, std::memory_order_release);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.M + CPW - 1) / CPW * S), 1, 1);
-  cfg.blockDim = dim3(ROWS_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
+  if (e != cudaSuccess) return e;
+  *count = cache[dev & 63].load(std::memory_order_acquire);
+  if (*count > 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t q = {};
+  q.gridDim = dim3(static_cast<unsigned>(device_sm_count() / S * S), 1, 1);
+  q.blockDim = dim3(ROWS_THREADS, 1, 1);
+  q.dynamicSmemBytes = Cfg::SMEM;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(S);
+  attr[0].val.clusterDim.x = S;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  q.attrs = attr;
+  q.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(count, kernel, &q);
+  if (e != cudaSuccess) return e;
+  if (*count < 1) return cudaErrorLaunchOutOfResources;
+  cache[dev & 63].store(*count, std::memory_order_release);
+  return cudaSuccess;
+}
+
+struct RowsCall {
+  const float* X; const float* W0; const float* W1;
+  float* out; float* G; float* U;
+  int N, M, K, act, early;
+};
+
+template <int NR, int MATS, int CPW, int S>
+int rows_launch(const RowsCall& c, cudaStream_t st) {
+  using Cfg = RowsCfg<NR, MATS, CPW, S>;
+  RowsParams p;
+  std::memset(&p, 0, sizeof(p));
+  if (int rc = make_map_rows(&p.tmW[0], c.W0, c.M, c.K, CPW, Cfg::KT)) return rc;
+  if (MATS == 2)
+    if (int rc = make_map_rows(&p.tmW[1], c.W1, c.M, c.K, CPW, Cfg::KT)) return rc;
+  if (int rc = make_map_rows(&p.tmX, c.X, c.K, c.N, Cfg::KT, NR)) return rc;
+  p.out = c.out; p.G = c.G; p.U = c.U;
+  p.N = c.N; p.M = c.M; p.act = c.act; p.early = c.early;
+  p.ktiles = (c.K + Cfg::KT - 1) / Cfg::KT;
+  p.items = (c.M + CPW - 1) / CPW;
+  cudaError_t e = rows_clusters<NR, MATS, CPW, S>(&p.clusters);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (p.clusters > p.items) p.clusters = p.items;
+  p.status = status_word_ptr(&e);
+  if (!p.status) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.clusters) * S, 1, 1);
+  cfg.blockDim = dim3(ROWS_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, p));
+  cfg.numAttrs = c.early ? 2 : 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, rows_kernel<NR, MATS, CPW, S>, p));
 }
 
-// Columns per cluster and CTAs per cluster: wide columns and few slices as long as they give every SM two CTAs.
+// Columns per item and blocks per cluster: what a block has to read (its items' tiles) decides, at 30 KB more per item for
+// the sums' way to their owner; on equal terms the wider columns (longer runs in memory).  Clusters of two use every SM;
+// clusters of four leave about a tenth idle (33 fit on 148 SMs).
 template <int NR, int MATS>
-int rows_launch(const RowsParams& p, cudaStream_t st) {
-  const int want = 2 * device_sm_count();
-  int cpw = 32, S = 8;
-  for (int c = 128; c >= 32 && cpw == 32; c >>= 1) {
-    const int blocks = (p.M + c - 1) / c;
-    for (int s = 1; s <= 8; s <<= 1)
-      if (blocks * s >= want && p.K / s >= 64) { cpw = c; S = s; break; }
-    if (cpw != 32 || (c == 32 && blocks * S >= want)) break;
+int rows_shape(const RowsCall& c, cudaStream_t st) {
+  const int sms = device_sm_count();
+  int best_w = 128, best_s = 1;
+  double best = 1e300;
+  for (int w = 128; w >= 32; w >>= 1)
+    for (int s = 1; s <= 4; s <<= 1) {
+      const int ktiles = (c.K * w + 4095) / 4096;
+      if (ktiles < s) continue;
+      const int items = (c.M + w - 1) / w, clusters = s == 4 ? sms * 2 / 9 : sms / s;
+      const double rounds = (items + clusters - 1) / clusters;
+      const double cost = rounds * (((ktiles + s - 1) / s) * MATS * 16384.0 + 30e3);
+      if (cost < best * 0.97) { best = cost; best_w = w; best_s = s; }
+    }
+  switch (best_w * 8 + best_s) {
+    case 128 * 8 + 1: return rows_launch<NR, MATS, 128, 1>(c, st);
+    case 128 * 8 + 2: return rows_launch<NR, MATS, 128, 2>(c, st);
+    case 128 * 8 + 4: return rows_launch<NR, MATS, 128, 4>(c, st);
+    case 64 * 8 + 1: return rows_launch<NR, MATS, 64, 1>(c, st);
+    case 64 * 8 + 2: return rows_launch<NR, MATS, 64, 2>(c, st);
+    case 64 * 8 + 4: return rows_launch<NR, MATS, 64, 4>(c, st);
+    case 32 * 8 + 1: return rows_launch<NR, MATS, 32, 1>(c, st);
+    case 32 * 8 + 2: return rows_launch<NR, MATS, 32, 2>(c, st);
+    default: return rows_launch<NR, MATS, 32, 4>(c, st);
   }
-  while (S > 1 && p.K / S < 16) S >>= 1;
-  if (cpw == 128) return rows_launch_one<NR, MATS, 128>(p, S, st);
-  if (cpw == 64) return rows_launch_one<NR, MATS, 64>(p, S, st);
-  return rows_launch_one<NR, MATS, 32>(p, S, st);
 }
 
-constexpr int ROWS_MAX = 16;
+constexpr int ROWS_MAX = 8;
 
 template <int MATS>
-int rows_any(const RowsParams& p, cudaStream_t st) {
-  if (p.N <= 1) return rows_launch<1, MATS>(p, st);
-  if (p.N <= 2) return rows_launch<2, MATS>(p, st);
-  if (p.N <= 4) return rows_launch<4, MATS>(p, st);
-  if (p.N <= 8) return rows_launch<8, MATS>(p, st);
-  return rows_launch<16, MATS>(p, st);
+int rows_any(const RowsCall& c, cudaStream_t st) {
+  if (!load_driver_entry_points()) return CU32_E_DRIVER;
+  if (c.N <= 1) return rows_shape<1, MATS>(c, st);
+  if (c.N <= 2) return rows_shape<2, MATS>(c, st);
+  if (c.N <= 4) return rows_shape<4, MATS>(c, st);
+  return rows_shape<8, MATS>(c, st);
 }
 
 // ------------------------------------------------------------------ many rows
@@ -412,14 +631,10 @@ int cu32_gatedFF(const int64_t* s, int length, const float* X, const float* Wg, 
   if (int rc = check_dims(N, D, F, act)) return rc;
   if (!all_aligned16(X, Wg, Wu, Wd, G, U, H, Y, work)) return CU32_E_ALIGN;
   if (N <= ROWS_MAX) {
-    RowsParams p{};
-    p.X = X; p.W[0] = Wg; p.W[1] = Wu; p.out = H; p.G = G; p.U = U;
-    p.N = N; p.M = F; p.K = D; p.act = act;
-    if (int rc = rows_any<2>(p, st)) return rc;
-    RowsParams q{};
-    q.X = H; q.W[0] = Wd; q.out = Y;
-    q.N = N; q.M = D; q.K = F;
-    return rows_any<1>(q, st);
+    const RowsCall up{X, Wg, Wu, H, G, U, N, F, D, act, 0};
+    if (int rc = rows_any<2>(up, st)) return rc;
+    const RowsCall down{H, Wd, nullptr, Y, nullptr, nullptr, N, D, F, 0, 1};
+    return rows_any<1>(down, st);
   }
   if (int rc = gated_tiles(X, Wg, Wu, G, U, H, N, D, F, act, st)) return rc;
   return product(s, false, true, H, F, Wd, D, Y, N, D, F, work, work_floats, st);

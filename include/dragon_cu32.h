@@ -433,7 +433,7 @@ CU32_API int cu32_batchMatMulT2_softmax(const int64_t* streams, int length, cons
  *   every base pointer 16-byte aligned.  act: one of CU32_ACT_*, applied to G.
  * cu32_gatedFF
  *   G and U are written for the gradient call when given; both null in serving.  H is always written.
- *   Up to 16 rows the weights are read once for all rows (FP32 multiply-adds); more rows run on the tensor cores, both
+ *   Up to 8 rows the weights are read once for all rows (FP32 multiply-adds); more rows run on the tensor cores, both
  *   projections, the activation and the product in one kernel.
  * cu32_gatedFF_delta
  *   deltaH = deltaY Wd^T, deltaG = deltaH * U * act'(G), deltaU = deltaH * act(G), both written (dG may be G and dU may
