@@ -31,6 +31,7 @@ struct GemmCall {
   float alpha = 1.0f;
   float* const* replicas = nullptr;   // further output buffers that receive the same stores as C (same layout)
   int n_replicas = 0;
+  bool beside_prev = false;           // may run beside the previous launch on the stream, which it does not depend on
 };
 
 int run_gemm(const GemmCall& c);

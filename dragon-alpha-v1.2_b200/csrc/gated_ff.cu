@@ -492,8 +492,10 @@ int sum_slices(int64_t stream, float* C, const float* Cbuf, int gz, long long si
 }
 
 // C[M,N] = op(A) op(B) through the plain contraction, cut along K where that pays.
+// beside: it may share the machine with the previous launch (whose last tiles leave SMs idle) - only where that launch
+// neither writes what this one reads nor reads what it writes, and the product is not cut (the scratch is one).
 int product(const int64_t* s, bool a_mn, bool b_mn, const float* A, long long lda, const float* B, long long ldb, float* C,
-            int M, int N, int K, float* work, long long room, cudaStream_t st) {
+            int M, int N, int K, float* work, long long room, cudaStream_t st, bool beside = false) {
   GemmCall c{};
   c.A = A; c.B = B; c.C = C; c.Cbuf = work;
   c.M = M; c.N = N; c.K = K; c.n_store = N;
@@ -501,6 +503,7 @@ int product(const int64_t* s, bool a_mn, bool b_mn, const float* A, long long ld
   c.batch = 1; c.sC = static_cast<long long>(M) * N;
   c.gz = split_of(PLAIN_TILES, 6, M, N, (K + 31) / 32, work ? room : 0);
   c.x3 = true; c.stream = st;
+  c.beside_prev = beside && c.gz == 1;
   if (int rc = run_gemm(c)) return rc;
   return sum_slices(s[0], C, work, c.gz, c.sC);
 }
@@ -520,46 +523,91 @@ int fill_common(GemmParams* p, int M, int N, int nkb, int tile, int out_bn) {
   return p->status ? CU32_OK : static_cast<int>(e);
 }
 
-// H = act(X Wg) * (X Wu) on the tensor cores, G and U stored when G is not null.
-int gated_tiles(const float* X, const float* Wg, const float* Wu, float* G, float* U, float* H, int N, int D, int F, int act,
-                cudaStream_t st) {
-  if (!load_driver_entry_points()) return CU32_E_DRIVER;
+// A gated launch covers its F columns in one piece, or in two: as many columns as fill whole rounds of 256x256 tiles on
+// the machine, and the rest in smaller tiles beside the last round (172 tiles are 2.3 rounds of 74 pairs: three rounds,
+// or two and a half-size one).  width: columns of the output per column of a tile (the gated form's tile holds two
+// columns per hidden unit).
+struct ColumnPlan { int first_cols, first_tile, rest_tile; };
+
+ColumnPlan plan_columns(long long M, int F, int nkb, int per_unit) {
+  ColumnPlan best{};
+  double best_t;
+  best.first_cols = F;
+  best.first_tile = best_tile(GATED_TILES, 3, M, static_cast<long long>(F) * per_unit, nkb, 1, &best_t);
+  if (forced_tile() >= 0) return best;
+  const int unit = 256 / per_unit;
+  const long long tiles_m = (M + 255) / 256, pairs = device_sm_count() / 2;
+  for (long long rounds = 1; rounds * pairs / tiles_m * unit < F; ++rounds) {
+    const int cols = static_cast<int>(rounds * pairs / tiles_m) * unit;
+    if (cols <= 0) continue;
+    double rest_t;
+    const int rest = best_tile(GATED_TILES, 3, M, static_cast<long long>(F - cols) * per_unit, nkb, 1, &rest_t);
+    const double t = tile_time(TILE_2x256, M, static_cast<long long>(cols) * per_unit, nkb, 1) + rest_t - 2e-6;
+    if (t < 0.97 * best_t) { best_t = t; best = ColumnPlan{cols, TILE_2x256, rest}; }
+  }
+  return best;
+}
+
+// H = act(X Wg) * (X Wu) on the tensor cores, G and U stored when G is not null: columns [c0, c0 + cols).
+int gated_part(const float* X, const float* Wg, const float* Wu, float* G, float* U, float* H, int N, int D, int F, int act,
+               int c0, int cols, int tile, bool beside, cudaStream_t st) {
   const int nkb = (D + 31) / 32;
-  const int tile = note_tile(best_tile(GATED_TILES, 3, N, 2LL * F, nkb, 1, nullptr));
+  note_tile(tile);
   GemmParams p;
   std::memset(&p, 0, sizeof(p));
-  const uint64_t n = N, d = D, f = F;
+  const uint64_t n = N, d = D, f = F, w = cols;
   if (int rc = make_map3(&p.tmA, X, d, n, 1, d, d * n, 32, 128, false)) return rc;
-  if (int rc = make_map3(&p.tmB, Wg, f, d, 1, f, f * d, 32, 32, true)) return rc;
-  if (int rc = make_map3(&p.tmRep[3], Wu, f, d, 1, f, f * d, 32, 32, true)) return rc;
-  if (int rc = make_map3(&p.tmC, H, f, n, 1, f, f * n, 32, 32, false)) return rc;
+  if (int rc = make_map3(&p.tmB, Wg + c0, w, d, 1, f, f * d, 32, 32, true)) return rc;
+  if (int rc = make_map3(&p.tmRep[3], Wu + c0, w, d, 1, f, f * d, 32, 32, true)) return rc;
+  if (int rc = make_map3(&p.tmC, H + c0, w, n, 1, f, f * n, 32, 32, false)) return rc;
   if (G) {
-    if (int rc = make_map3(&p.tmRep[0], G, f, n, 1, f, f * n, 32, 32, false)) return rc;
-    if (int rc = make_map3(&p.tmRep[1], U, f, n, 1, f, f * n, 32, 32, false)) return rc;
+    if (int rc = make_map3(&p.tmRep[0], G + c0, w, n, 1, f, f * n, 32, 32, false)) return rc;
+    if (int rc = make_map3(&p.tmRep[1], U + c0, w, n, 1, f, f * n, 32, 32, false)) return rc;
     p.gated_save = 1;
   }
-  if (int rc = fill_common(&p, N, F, nkb, tile, tile_bn(tile) / 2)) return rc;
-  p.C = H; p.act = act; p.tma_store = 1;
+  if (int rc = fill_common(&p, N, cols, nkb, tile, tile_bn(tile) / 2)) return rc;
+  p.C = H + c0; p.ldc = F; p.act = act; p.tma_store = 1;
+  p.overlap_prev = p.join_prev = beside ? 1 : 0;
   p.flush_chunks = nkb;      // one flush: the activation needs the complete sums
   return static_cast<int>(launch_gemm_gated(tile, p, st));
 }
 
-// deltaG, deltaU from deltaY, Wd, G, U.
-int dgated_tiles(const float* dY, const float* Wd, const float* G, const float* U, float* dG, float* dU, int N, int D, int F,
-                 int act, cudaStream_t st) {
+int gated_tiles(const float* X, const float* Wg, const float* Wu, float* G, float* U, float* H, int N, int D, int F, int act,
+                cudaStream_t st) {
   if (!load_driver_entry_points()) return CU32_E_DRIVER;
+  const ColumnPlan c = plan_columns(N, F, (D + 31) / 32, 2);
+  if (int rc = gated_part(X, Wg, Wu, G, U, H, N, D, F, act, 0, c.first_cols, c.first_tile, false, st)) return rc;
+  if (c.first_cols == F) return CU32_OK;
+  return gated_part(X, Wg, Wu, G, U, H, N, D, F, act, c.first_cols, F - c.first_cols, c.rest_tile, true, st);
+}
+
+// deltaG, deltaU from deltaY, Wd, G, U: columns [c0, c0 + cols).
+int dgated_part(const float* dY, const float* Wd, const float* G, const float* U, float* dG, float* dU, int N, int D, int F,
+                int act, int c0, int cols, int tile, bool beside, cudaStream_t st) {
   const int nkb = (D + 31) / 32;
-  const int tile = note_tile(best_tile(GATED_TILES, 3, N, F, nkb, 1, nullptr));
+  note_tile(tile);
   GemmParams p;
   std::memset(&p, 0, sizeof(p));
-  const uint64_t n = N, d = D, f = F;
+  const uint64_t n = N, d = D, w = cols;
   if (int rc = make_map3(&p.tmA, dY, d, n, 1, d, d * n, 32, 128, false)) return rc;
-  if (int rc = make_map3(&p.tmB, Wd, d, f, 1, d, d * f, 32, tile_bn(tile) / tile_ctas(tile), false)) return rc;
-  if (int rc = fill_common(&p, N, F, nkb, tile, tile_bn(tile))) return rc;
-  p.C = dG; p.act = act;
-  p.ep_g = G; p.ep_u = U; p.ep_dg = dG; p.ep_du = dU;
+  if (int rc = make_map3(&p.tmB, Wd + static_cast<long long>(c0) * D, d, w, 1, d, d * w, 32, tile_bn(tile) / tile_ctas(tile), false))
+    return rc;
+  if (int rc = fill_common(&p, N, cols, nkb, tile, tile_bn(tile))) return rc;
+  p.C = dG + c0; p.ldc = F; p.act = act;
+  p.ep_g = G + c0; p.ep_u = U + c0; p.ep_dg = dG + c0; p.ep_du = dU + c0;
+  p.overlap_prev = p.join_prev = beside ? 1 : 0;
   p.flush_chunks = nkb;
   return static_cast<int>(launch_gemm_dgated(tile, p, st));
+}
+
+// beside: it may run beside the previous launch.
+int dgated_tiles(const float* dY, const float* Wd, const float* G, const float* U, float* dG, float* dU, int N, int D, int F,
+                 int act, bool beside, cudaStream_t st) {
+  if (!load_driver_entry_points()) return CU32_E_DRIVER;
+  const ColumnPlan c = plan_columns(N, F, (D + 31) / 32, 1);
+  if (int rc = dgated_part(dY, Wd, G, U, dG, dU, N, D, F, act, 0, c.first_cols, c.first_tile, beside, st)) return rc;
+  if (c.first_cols == F) return CU32_OK;
+  return dgated_part(dY, Wd, G, U, dG, dU, N, D, F, act, c.first_cols, F - c.first_cols, c.rest_tile, true, st);
 }
 
 // deltaX = deltaG Wg^T + deltaU Wu^T
@@ -650,15 +698,17 @@ int cu32_gatedFF_delta(const int64_t* s, int length, const float* dY, const floa
   if ((dX && any_null(Wg, Wu)) || ((dWg || dWu) && !X) || (dWd && !H)) return CU32_E_NULL;
   if (int rc = check_dims(N, D, F, act)) return rc;
   if (!all_aligned16(dY, X, Wg, Wu, Wd, G, U, H, dG, dU, dX, dWg, dWu, dWd, work)) return CU32_E_ALIGN;
+  // Launches that do not depend on each other stand side by side, so that the tiles of the next fill the last round of
+  // the one before: deltaWd with deltaG / deltaU, and deltaWg with deltaWu.
   if (dWd)
     if (int rc = product(s, true, true, H, F, dY, D, dWd, F, D, N, work, work_floats, st)) return rc;
-  if (int rc = dgated_tiles(dY, Wd, G, U, dG, dU, N, D, F, act, st)) return rc;
+  if (int rc = dgated_tiles(dY, Wd, G, U, dG, dU, N, D, F, act, dWd != nullptr, st)) return rc;
   if (dX)
     if (int rc = dual_tiles(s, dG, Wg, dU, Wu, dX, N, D, F, work, work_floats, st)) return rc;
   if (dWg)
-    if (int rc = product(s, true, true, X, D, dG, F, dWg, D, F, N, work, work_floats, st)) return rc;
+    if (int rc = product(s, true, true, X, D, dG, F, dWg, D, F, N, work, work_floats, st, false)) return rc;
   if (dWu)
-    if (int rc = product(s, true, true, X, D, dU, F, dWu, D, F, N, work, work_floats, st)) return rc;
+    if (int rc = product(s, true, true, X, D, dU, F, dWu, D, F, N, work, work_floats, st, dWg != nullptr)) return rc;
   return CU32_OK;
 }
 

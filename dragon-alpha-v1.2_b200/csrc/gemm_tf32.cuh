@@ -110,6 +110,8 @@ struct GemmParams {
   int arrive_release;   // debugging aid: remote mbarrier arrives carry a cluster-scope release
   int overlap_prev;     // host side only: this launch may start while the previous launch on the stream is still
                         // running (it does not depend on its results - the phases of a strided data gradient)
+  int join_prev;        // with overlap_prev: no block leaves before the previous launch has ended, so whoever waits for this
+                        // launch has waited for that one too
   int sm_reserve;       // SMs the persistent grid leaves free (for a collective's kernels running beside it)
   // im2col geometry (A gathered from an NHWC feature map); unused otherwise.
   // The reduction index runs over (fh, fw, ic) with every filter tap padded to
@@ -1338,6 +1340,7 @@ __device__ __forceinline__ void gemm_tf32_body(const GemmParams& p) {
   }
 
   // ---- common exit: everyone arrives here, also after a give-up
+  if (p.join_prev) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   if (p.clock_acc != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
