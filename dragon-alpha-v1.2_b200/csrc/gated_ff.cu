@@ -474,11 +474,10 @@ const int DUAL_TILES[4] = {TILE_1x64, TILE_1x128, TILE_2x128, TILE_2x256};
 const int PLAIN_TILES[6] = {TILE_1x64, TILE_1x128, TILE_1x256, TILE_2x128, TILE_2x256, TILE_2x64};
 
 // Slices of the reduction for an [M, N] product when `room` floats of partial sums are at hand.
-int split_of(const int* tiles, int count, long long M, long long N, int nkb, long long room) {
-  static const int cuts[] = {1, 2, 3, 4, 6, 8, 12, 16};
+int split_of(const int* tiles, int count, long long M, long long N, int nkb, long long room, double uncut = 1e300) {
   int best = 1;
-  double best_t = 1e300;
-  for (int gz : cuts) {
+  double best_t = uncut;      // what the product takes in one piece by another plan, where there is one
+  for (int gz = 1; gz <= 16; ++gz) {
     if (gz > 1 && (nkb / gz < 4 || (gz - 1) * M * N > room)) break;
     double t;
     best_tile(tiles, count, M, N, nkb, gz, &t);
@@ -491,9 +490,34 @@ int sum_slices(int64_t stream, float* C, const float* Cbuf, int gz, long long si
   return gz > 1 ? cu32_SKbuf_summary(stream, Cbuf, C, gz - 1, static_cast<int>(size)) : CU32_OK;
 }
 
-// C[M,N] = op(A) op(B) through the plain contraction, cut along K where that pays.
+// A launch covers its columns in one piece, or in two: as many columns as fill whole rounds of 256x256 tiles on the
+// machine, and the rest in smaller tiles beside the last round (172 tiles are 2.3 rounds of 74 pairs: three rounds, or two
+// and a half-size one).  per_unit: tile columns per output column (the gated form's tile holds two per hidden unit).
+struct ColumnPlan { int first_cols, first_tile, rest_tile; double time; };
+
+ColumnPlan plan_columns(const int* tiles, int count, long long M, int N, int nkb, int per_unit) {
+  ColumnPlan best{};
+  double best_t;
+  best.first_cols = N;
+  best.first_tile = best_tile(tiles, count, M, static_cast<long long>(N) * per_unit, nkb, 1, &best_t);
+  best.time = best_t;
+  if (forced_tile() >= 0) return best;
+  const int unit = 256 / per_unit;
+  const long long tiles_m = (M + 255) / 256, pairs = device_sm_count() / 2;
+  for (long long rounds = 1; rounds * pairs / tiles_m * unit < N; ++rounds) {
+    const int cols = static_cast<int>(rounds * pairs / tiles_m) * unit;
+    if (cols <= 0) continue;
+    double rest_t;
+    const int rest = best_tile(tiles, count, M, static_cast<long long>(N - cols) * per_unit, nkb, 1, &rest_t);
+    const double t = tile_time(TILE_2x256, M, static_cast<long long>(cols) * per_unit, nkb, 1) + rest_t - 2e-6;
+    if (t < 0.97 * best_t) { best_t = t; best = ColumnPlan{cols, TILE_2x256, rest, t}; }
+  }
+  return best;
+}
+
+// C[M,N] = op(A) op(B) through the plain contraction, cut along K or along its columns where that pays.
 // beside: it may share the machine with the previous launch (whose last tiles leave SMs idle) - only where that launch
-// neither writes what this one reads nor reads what it writes, and the product is not cut (the scratch is one).
+// neither writes what this one reads nor reads what it writes, and the product is not cut along K (the scratch is one).
 int product(const int64_t* s, bool a_mn, bool b_mn, const float* A, long long lda, const float* B, long long ldb, float* C,
             int M, int N, int K, float* work, long long room, cudaStream_t st, bool beside = false) {
   GemmCall c{};
@@ -501,11 +525,23 @@ int product(const int64_t* s, bool a_mn, bool b_mn, const float* A, long long ld
   c.M = M; c.N = N; c.K = K; c.n_store = N;
   c.lda = lda; c.ldb = ldb; c.ldc = N; c.a_mn = a_mn; c.b_mn = b_mn;
   c.batch = 1; c.sC = static_cast<long long>(M) * N;
-  c.gz = split_of(PLAIN_TILES, 6, M, N, (K + 31) / 32, work ? room : 0);
+  const int nkb = (K + 31) / 32;
+  const ColumnPlan plan = plan_columns(PLAIN_TILES, 6, M, N, nkb, 1);
+  c.gz = split_of(PLAIN_TILES, 6, M, N, nkb, work ? room : 0, plan.time);
   c.x3 = true; c.stream = st;
   c.beside_prev = beside && c.gz == 1;
+  if (c.gz > 1) {
+    if (int rc = run_gemm(c)) return rc;
+    return sum_slices(s[0], C, work, c.gz, c.sC);
+  }
+  c.N = c.n_store = plan.first_cols;
   if (int rc = run_gemm(c)) return rc;
-  return sum_slices(s[0], C, work, c.gz, c.sC);
+  if (plan.first_cols == N) return CU32_OK;
+  c.B = b_mn ? B + plan.first_cols : B + plan.first_cols * ldb;
+  c.C = C + plan.first_cols;
+  c.N = c.n_store = N - plan.first_cols;
+  c.beside_prev = true;
+  return run_gemm(c);
 }
 
 // What every launch of the contraction kernel needs besides its operand maps.
@@ -521,31 +557,6 @@ int fill_common(GemmParams* p, int M, int N, int nkb, int tile, int out_bn) {
   cudaError_t e;
   p->status = status_word_ptr(&e);
   return p->status ? CU32_OK : static_cast<int>(e);
-}
-
-// A gated launch covers its F columns in one piece, or in two: as many columns as fill whole rounds of 256x256 tiles on
-// the machine, and the rest in smaller tiles beside the last round (172 tiles are 2.3 rounds of 74 pairs: three rounds,
-// or two and a half-size one).  width: columns of the output per column of a tile (the gated form's tile holds two
-// columns per hidden unit).
-struct ColumnPlan { int first_cols, first_tile, rest_tile; };
-
-ColumnPlan plan_columns(long long M, int F, int nkb, int per_unit) {
-  ColumnPlan best{};
-  double best_t;
-  best.first_cols = F;
-  best.first_tile = best_tile(GATED_TILES, 3, M, static_cast<long long>(F) * per_unit, nkb, 1, &best_t);
-  if (forced_tile() >= 0) return best;
-  const int unit = 256 / per_unit;
-  const long long tiles_m = (M + 255) / 256, pairs = device_sm_count() / 2;
-  for (long long rounds = 1; rounds * pairs / tiles_m * unit < F; ++rounds) {
-    const int cols = static_cast<int>(rounds * pairs / tiles_m) * unit;
-    if (cols <= 0) continue;
-    double rest_t;
-    const int rest = best_tile(GATED_TILES, 3, M, static_cast<long long>(F - cols) * per_unit, nkb, 1, &rest_t);
-    const double t = tile_time(TILE_2x256, M, static_cast<long long>(cols) * per_unit, nkb, 1) + rest_t - 2e-6;
-    if (t < 0.97 * best_t) { best_t = t; best = ColumnPlan{cols, TILE_2x256, rest}; }
-  }
-  return best;
 }
 
 // H = act(X Wg) * (X Wu) on the tensor cores, G and U stored when G is not null: columns [c0, c0 + cols).
@@ -575,39 +586,37 @@ int gated_part(const float* X, const float* Wg, const float* Wu, float* G, float
 int gated_tiles(const float* X, const float* Wg, const float* Wu, float* G, float* U, float* H, int N, int D, int F, int act,
                 cudaStream_t st) {
   if (!load_driver_entry_points()) return CU32_E_DRIVER;
-  const ColumnPlan c = plan_columns(N, F, (D + 31) / 32, 2);
+  const ColumnPlan c = plan_columns(GATED_TILES, 3, N, F, (D + 31) / 32, 2);
   if (int rc = gated_part(X, Wg, Wu, G, U, H, N, D, F, act, 0, c.first_cols, c.first_tile, false, st)) return rc;
   if (c.first_cols == F) return CU32_OK;
   return gated_part(X, Wg, Wu, G, U, H, N, D, F, act, c.first_cols, F - c.first_cols, c.rest_tile, true, st);
 }
 
-// deltaG, deltaU from deltaY, Wd, G, U: columns [c0, c0 + cols).
-int dgated_part(const float* dY, const float* Wd, const float* G, const float* U, float* dG, float* dU, int N, int D, int F,
-                int act, int c0, int cols, int tile, bool beside, cudaStream_t st) {
-  const int nkb = (D + 31) / 32;
-  note_tile(tile);
-  GemmParams p;
-  std::memset(&p, 0, sizeof(p));
-  const uint64_t n = N, d = D, w = cols;
-  if (int rc = make_map3(&p.tmA, dY, d, n, 1, d, d * n, 32, 128, false)) return rc;
-  if (int rc = make_map3(&p.tmB, Wd + static_cast<long long>(c0) * D, d, w, 1, d, d * w, 32, tile_bn(tile) / tile_ctas(tile), false))
-    return rc;
-  if (int rc = fill_common(&p, N, cols, nkb, tile, tile_bn(tile))) return rc;
-  p.C = dG + c0; p.ldc = F; p.act = act;
-  p.ep_g = G + c0; p.ep_u = U + c0; p.ep_dg = dG + c0; p.ep_du = dU + c0;
-  p.overlap_prev = p.join_prev = beside ? 1 : 0;
-  p.flush_chunks = nkb;
-  return static_cast<int>(launch_gemm_dgated(tile, p, st));
-}
-
-// beside: it may run beside the previous launch.
-int dgated_tiles(const float* dY, const float* Wd, const float* G, const float* U, float* dG, float* dU, int N, int D, int F,
-                 int act, bool beside, cudaStream_t st) {
-  if (!load_driver_entry_points()) return CU32_E_DRIVER;
-  const ColumnPlan c = plan_columns(N, F, (D + 31) / 32, 1);
-  if (int rc = dgated_part(dY, Wd, G, U, dG, dU, N, D, F, act, 0, c.first_cols, c.first_tile, beside, st)) return rc;
-  if (c.first_cols == F) return CU32_OK;
-  return dgated_part(dY, Wd, G, U, dG, dU, N, D, F, act, c.first_cols, F - c.first_cols, c.rest_tile, true, st);
+// deltaG = deltaH * U * act'(G) and deltaU = deltaH * act(G), deltaH read where deltaG is written.  A pass of its own
+// (five floats per element, 36 us for 2048 x 5464): as the epilogue of deltaH's product it took more than it saved,
+// because a tile's epilogue stands in the way of the next tile's products (two rounds of K = 2048 tiles: 135 us as
+// straight-line code, waiting for instructions; 102 us as a loop; 64 us for the plain product).
+// Each thread reads its elements before it writes them, so deltaU may lie over G or U.
+__global__ void __launch_bounds__(256) gated_delta_kernel(float* dG, float* dU, const float* G, const float* U, long long vecs,
+                                                          int act) {
+  const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long v = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; v < vecs; v += 2 * stride) {
+    const bool two = v + stride < vecs;
+    const long long w = two ? v + stride : v;
+    const float4 d0 = reinterpret_cast<const float4*>(dG)[v], g0 = reinterpret_cast<const float4*>(G)[v],
+                 u0 = reinterpret_cast<const float4*>(U)[v];
+    const float4 d1 = reinterpret_cast<const float4*>(dG)[w], g1 = reinterpret_cast<const float4*>(G)[w],
+                 u1 = reinterpret_cast<const float4*>(U)[w];
+    float4 a, b;
+    gated_backward4(act, d0, g0, u0, &a, &b);
+    reinterpret_cast<float4*>(dG)[v] = a;
+    reinterpret_cast<float4*>(dU)[v] = b;
+    if (two) {
+      gated_backward4(act, d1, g1, u1, &a, &b);
+      reinterpret_cast<float4*>(dG)[w] = a;
+      reinterpret_cast<float4*>(dU)[w] = b;
+    }
+  }
 }
 
 // deltaX = deltaG Wg^T + deltaU Wu^T
@@ -695,14 +704,20 @@ int cu32_gatedFF_delta(const int64_t* s, int length, const float* dY, const floa
   cudaStream_t st;
   if (int rc = check_streams(s, length, &st)) return rc;
   if (any_null(dY, Wd, G, U, dG, dU)) return CU32_E_NULL;
+  if (dG == G || dG == U || dG == dU) return CU32_E_ARG;      // deltaH is formed where deltaG will be
   if ((dX && any_null(Wg, Wu)) || ((dWg || dWu) && !X) || (dWd && !H)) return CU32_E_NULL;
   if (int rc = check_dims(N, D, F, act)) return rc;
   if (!all_aligned16(dY, X, Wg, Wu, Wd, G, U, H, dG, dU, dX, dWg, dWu, dWd, work)) return CU32_E_ALIGN;
   // Launches that do not depend on each other stand side by side, so that the tiles of the next fill the last round of
-  // the one before: deltaWd with deltaG / deltaU, and deltaWg with deltaWu.
+  // the one before: deltaWd with deltaH, and deltaWg with deltaWu.
   if (dWd)
     if (int rc = product(s, true, true, H, F, dY, D, dWd, F, D, N, work, work_floats, st)) return rc;
-  if (int rc = dgated_tiles(dY, Wd, G, U, dG, dU, N, D, F, act, dWd != nullptr, st)) return rc;
+  if (int rc = product(s, false, false, dY, D, Wd, D, dG, N, F, D, work, work_floats, st, dWd != nullptr && dG != H)) return rc;
+  const long long vecs = static_cast<long long>(N) * F / 4;
+  long long blocks = (vecs + 511) / 512;
+  if (blocks > 16LL * device_sm_count()) blocks = 16LL * device_sm_count();
+  gated_delta_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(dG, dU, G, U, vecs, act);
+  if (cudaError_t e = cudaPeekAtLastError()) return static_cast<int>(e);
   if (dX)
     if (int rc = dual_tiles(s, dG, Wg, dU, Wu, dX, N, D, F, work, work_floats, st)) return rc;
   if (dWg)

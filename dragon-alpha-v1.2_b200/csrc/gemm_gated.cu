@@ -1,5 +1,4 @@
-// Kernel instantiations of the gated feed-forward block: act(A*B) * (A*B2) with A[M][K], B[K][N]; deltaH = A*B^T turned
-// into deltaG and deltaU; and the sum of two products A*B^T + A2*B2^T.
+// Kernel instantiations of the gated feed-forward block's first half: act(A*B) * (A*B2) with A[M][K], B[K][N].
 #include "gemm_launch.h"
 
 namespace dragon {
@@ -10,16 +9,6 @@ cudaError_t launch_gemm_gated(int tile_cfg, const GemmParams& p, cudaStream_t st
     case TILE_1x128: return launch_one<GemmCfg<128, 1, false, true, true, false, false, false, EPI_GATED>>(p, grid_z, stream);
     case TILE_2x128: return launch_one<GemmCfg<128, 2, false, true, true, false, false, false, EPI_GATED>>(p, grid_z, stream);
     case TILE_2x256: return launch_one<GemmCfg<256, 2, false, true, true, false, false, false, EPI_GATED>>(p, grid_z, stream);
-    default: return cudaErrorInvalidValue;
-  }
-}
-
-cudaError_t launch_gemm_dgated(int tile_cfg, const GemmParams& p, cudaStream_t stream) {
-  const int grid_z = 1;
-  switch (tile_cfg) {
-    case TILE_1x128: return launch_one<GemmCfg<128, 1, false, false, true, false, false, false, EPI_DGATED>>(p, grid_z, stream);
-    case TILE_2x128: return launch_one<GemmCfg<128, 2, false, false, true, false, false, false, EPI_DGATED>>(p, grid_z, stream);
-    case TILE_2x256: return launch_one<GemmCfg<256, 2, false, false, true, false, false, false, EPI_DGATED>>(p, grid_z, stream);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -59,10 +59,9 @@ cudaError_t launch_gemm_rep(bool b_mn, const GemmParams& p, int grid_z, cudaStre
 cudaError_t launch_gemm_nn_im2col(int tile_cfg, const GemmParams& p, int grid_z, cudaStream_t stream);
 
 // The gated feed-forward block, FP32-accurate, tiles TILE_1x128, TILE_2x128, TILE_2x256 (dual also TILE_1x64):
-//   gated  : C = act(A * B) * (A * B2), KN layouts;   dgated: deltaG, deltaU from deltaH = A * B^T, KK layouts
+//   gated  : C = act(A * B) * (A * B2), KN layouts
 //   dual   : C = A * B^T + A2 * B2^T, KK layouts (grid_z > 1: split-K slices)
 cudaError_t launch_gemm_gated(int tile_cfg, const GemmParams& p, cudaStream_t stream);
-cudaError_t launch_gemm_dgated(int tile_cfg, const GemmParams& p, cudaStream_t stream);
 cudaError_t launch_gemm_dual(int tile_cfg, const GemmParams& p, int grid_z, cudaStream_t stream);
 
 template <class Cfg>

@@ -145,18 +145,13 @@ struct GemmParams {
   int act;              // activation, CU32_ACT_*
   int gated_save;       // EPI_GATED: store G and U too
   int nkb_first;        // EPI_DUAL: k-blocks of the first product; the rest belong to the second
-  const float* ep_g;    // EPI_DGATED: G, U [M, N] read, deltaG, deltaU written, all with C's pitch (the outputs may
-  const float* ep_u;    // be the inputs' own buffers)
-  float* ep_dg;
-  float* ep_du;
 };
 
 // What happens to a finished tile beyond the plain store:
 //   EPI_GATED   the tile's columns are two interleaved products A*B and A*B2 of the same hidden units: act(G) * U is
 //               stored (and G and U, when asked), a tile covers BN / 2 hidden units
-//   EPI_DGATED  the tile is deltaH: deltaG = deltaH * U * act'(G) and deltaU = deltaH * act(G) are stored instead
 //   EPI_DUAL    C = A*B + A2*B2, the second product's k-blocks behind the first's
-enum GemmEpilogue : int { EPI_NONE = 0, EPI_GATED = 1, EPI_DGATED = 2, EPI_DUAL = 3 };
+enum GemmEpilogue : int { EPI_NONE = 0, EPI_GATED = 1, EPI_DUAL = 2 };
 
 enum GemmRole : int { ROLE_TMA = 1, ROLE_SPLIT = 2, ROLE_MMA = 3, ROLE_MMA_TMEM = 4, ROLE_DRAIN = 5, ROLE_SELFTEST = 7 };
 
@@ -173,8 +168,7 @@ struct GemmCfg {
   static constexpr bool REP = REP_;
   static constexpr int EPI = EPI_;
   static_assert(EPI_ != EPI_GATED || (!A_MN_ && B_MN_ && X3_ && !IM2COL_ && BN_ >= 128), "gated: A[M][K] x B[K][N]");
-  static_assert((EPI_ != EPI_DGATED && EPI_ != EPI_DUAL) || (!A_MN_ && !B_MN_ && X3_ && !IM2COL_),
-                "gated gradients: A[M][K] x B[N][K]^T");
+  static_assert(EPI_ != EPI_DUAL || (!A_MN_ && !B_MN_ && X3_ && !IM2COL_), "dual: A[M][K] x B[N][K]^T");
   static constexpr int OUT_BN = EPI_ == EPI_GATED ? BN_ / 2 : BN_;   // output columns of a tile
   static_assert(!SOFTMAX_ || (BN_ == 256 && CTAS_ == 2 && X3_ && !A_MN_ && !B_MN_ && !IM2COL_),
                 "the row softmax is built on the 256x256 pair tile of the A * B^T form");
@@ -1157,51 +1151,6 @@ __device__ __forceinline__ void gemm_tf32_body(const GemmParams& p) {
           for (int g = 0; g < HW / 32; ++g) {
             const int c0 = w.col0 + h * HW + g * 32;
             if (c0 < p.N && r0 < p.M) put(&p.tmC, g * 32, c0);
-          }
-        } else if constexpr (Cfg::EPI == EPI_DGATED) {
-          // deltaH never leaves the SM: each 32x32 piece goes through the staging tile so that eight lanes share a
-          // row's 128 bytes (whole segments of G, U, deltaG and deltaU), and the elementwise part happens there.
-          const uint32_t stg = stg0;
-          const int sub = lane >> 3, chunk = lane & 7;
-#pragma unroll
-          for (int g = 0; g < CW / 32; ++g) {
-            const int c0 = w.col0 + h * CW + g * 32;
-            if (c0 < p.N && w.row0 + q * 32 < p.M) {   // warp-uniform
-#pragma unroll
-              for (int cq = 0; cq < 8; ++cq)
-                sts128(stg + lane * 128 + ((cq ^ (lane & 7)) * 16),
-                       make_float4(acc[g * 32 + cq * 4], acc[g * 32 + cq * 4 + 1], acc[g * 32 + cq * 4 + 2],
-                                   acc[g * 32 + cq * 4 + 3]));
-              __syncwarp();
-              const bool col_ok = c0 + chunk * 4 < p.N;   // p.N is a multiple of 4: a vector is whole or absent
-              const long long off0 = static_cast<long long>(w.row0 + q * 32 + sub) * p.ldc + c0 + chunk * 4;
-#pragma unroll
-              for (int i0 = 0; i0 < 8; i0 += 2) {
-                float4 gv[2], uv[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  const int r = (i0 + i) * 4 + sub;
-                  if (col_ok && w.row0 + q * 32 + r < p.M) {
-                    const long long off = off0 + static_cast<long long>(i0 + i) * 4 * p.ldc;
-                    gv[i] = *reinterpret_cast<const float4*>(p.ep_g + off);
-                    uv[i] = *reinterpret_cast<const float4*>(p.ep_u + off);
-                  }
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  const int r = (i0 + i) * 4 + sub;
-                  if (col_ok && w.row0 + q * 32 + r < p.M) {
-                    const long long off = off0 + static_cast<long long>(i0 + i) * 4 * p.ldc;
-                    const float4 d = lds128(stg + r * 128 + ((chunk ^ (r & 7)) * 16));
-                    float4 dg, du;
-                    gated_backward4(p.act, d, gv[i], uv[i], &dg, &du);
-                    *reinterpret_cast<float4*>(p.ep_dg + off) = dg;
-                    *reinterpret_cast<float4*>(p.ep_du + off) = du;
-                  }
-                }
-              }
-              __syncwarp();   // the piece has been read before the next one overwrites it
-            }
           }
         } else if (use_tma) {
           // Each drain warp owns a 32-row x CW-column block.  32x32 pieces go through a

@@ -436,8 +436,8 @@ CU32_API int cu32_batchMatMulT2_softmax(const int64_t* streams, int length, cons
  *   Up to 8 rows the weights are read once for all rows (FP32 multiply-adds); more rows run on the tensor cores, both
  *   projections, the activation and the product in one kernel.
  * cu32_gatedFF_delta
- *   deltaH = deltaY Wd^T, deltaG = deltaH * U * act'(G), deltaU = deltaH * act(G), both written (dG may be G and dU may
- *   be U: they are then replaced); deltaX = deltaG Wg^T + deltaU Wu^T, deltaWg = X^T deltaG, deltaWu = X^T deltaU,
+ *   deltaH = deltaY Wd^T, deltaG = deltaH * U * act'(G), deltaU = deltaH * act(G), both written; deltaU may be G or U and
+ *   deltaG may be H, which are then replaced (deltaG must not be G, U or deltaU: CU32_E_ARG); deltaX = deltaG Wg^T + deltaU Wu^T, deltaWg = X^T deltaG, deltaWu = X^T deltaU,
  *   deltaWd = H^T deltaY.  deltaX, deltaWg, deltaWu and deltaWd may each be null: that gradient is not computed (and
  *   the operands only it needs may be null).
  * work: work_floats floats of scratch for split reductions, or null / 0 (products are then not split); its contents

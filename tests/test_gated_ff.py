@@ -75,12 +75,13 @@ class Block:
                                       self.Y.ptr, work.data_ptr() if work is not None else 0,
                                       work.numel() if work is not None else 0, self.N, self.D, self.F, act)
 
-    def backward(self, pkg, act, work=None, in_place=False):
+    def backward(self, pkg, act, work=None, over=None):
+        """over: "U" or "G" - deltaG lies over H, deltaU over U or G."""
         import gpu_util as G
         pkg.cu32.Cuda_gatedFF.gatedFF_delta(
             [G.stream()], 1, self.dY.data_ptr(), self.X.data_ptr(), self.Wg.data_ptr(), self.Wu.data_ptr(),
-            self.Wd.data_ptr(), self.G.ptr, self.U.ptr, self.H.ptr, self.G.ptr if in_place else self.dG.ptr,
-            self.U.ptr if in_place else self.dU.ptr, self.dX.ptr, self.dWg.ptr, self.dWu.ptr, self.dWd.ptr,
+            self.Wd.data_ptr(), self.G.ptr, self.U.ptr, self.H.ptr, self.H.ptr if over else self.dG.ptr,
+            getattr(self, over).ptr if over else self.dU.ptr, self.dX.ptr, self.dWg.ptr, self.dWu.ptr, self.dWd.ptr,
             work.data_ptr() if work is not None else 0, work.numel() if work is not None else 0, self.N, self.D, self.F, act)
 
     def get(self, torch, name):
@@ -123,8 +124,8 @@ def test_gated_ff_refusals(pkg):
     def fwd(X=P, Wg=P, Wu=P, Wd=P, G=0, U=0, H=P, Y=P, work=0, room=0, N=4, D=8, F=12, act=0, length=1):
         return lib.cu32_gatedFF(s, length, X, Wg, Wu, Wd, G, U, H, Y, work, room, N, D, F, act)
 
-    def bwd(dY=P, X=P, Wg=P, Wu=P, Wd=P, G=P, U=P, H=P, dG=P, dU=P, dX=P, dWg=P, dWu=P, dWd=P, work=0, room=0, N=4, D=8, F=12,
-            act=0, length=1):
+    def bwd(dY=P, X=P, Wg=P, Wu=P, Wd=P, G=P, U=P, H=P, dG=2 * P, dU=P, dX=P, dWg=P, dWu=P, dWd=P, work=0, room=0, N=4, D=8,
+            F=12, act=0, length=1):
         return lib.cu32_gatedFF_delta(s, length, dY, X, Wg, Wu, Wd, G, U, H, dG, dU, dX, dWg, dWu, dWd, work, room, N, D, F, act)
     for call in (fwd, bwd):
         assert call(length=0) == -3 and call(length=11) == -3
@@ -142,6 +143,8 @@ def test_gated_ff_refusals(pkg):
         assert bwd(**{name: 0}) == -1
     assert bwd(Wg=0) == -1 and bwd(X=0) == -1 and bwd(H=0) == -1
     assert bwd(X=0, dWg=0) == -1                                # deltaWu still needs X
+    Q = 2 * P
+    assert bwd(G=Q) == -8 and bwd(U=Q) == -8 and bwd(dU=Q) == -8 and bwd(dG=P) == -8    # deltaG over G, U or deltaU
     for name in ("dY", "X", "Wg", "Wu", "Wd", "G", "U", "H", "dG", "dU", "dX", "dWg", "dWu", "dWd"):
         assert bwd(**{name: P + 4}) == -4
     with pytest.raises(pkg.cu32.CudaException, match="CU32_E_NULL"):
@@ -217,21 +220,24 @@ def test_long_reductions(pkg, cuda, shape):
 
 @pytest.mark.gpu
 def test_gradients_in_place_and_single_ones(pkg, cuda):
-    """deltaG over G and deltaU over U give the bits of separate buffers; gradients that are not asked for are skipped,
-    with the operands only they need absent."""
+    """deltaG over H and deltaU over U or G give the bits of separate buffers; gradients that are not asked for are
+    skipped, with the operands only they need absent."""
     import gpu_util as G
     torch = cuda
     b = Block(torch, 70, 132, 196, seed=5)
     b.forward(pkg, 1)
-    keep_G, keep_U = b.G.view.clone(), b.U.view.clone()
+    kept = {n: getattr(b, n).view.clone() for n in "GUH"}
     b.backward(pkg, 1)
     first = {n: b.get(torch, n) for n in ("dG", "dU", "dX", "dWg", "dWu", "dWd")}
-    b.backward(pkg, 1, in_place=True)
-    assert torch.equal(b.get(torch, "G"), first["dG"]) and torch.equal(b.get(torch, "U"), first["dU"])
-    for n in ("dX", "dWg", "dWu", "dWd"):
-        assert torch.equal(b.get(torch, n), first[n])
-    b.G.view.copy_(keep_G)
-    b.U.view.copy_(keep_U)
+    for over in "UG":
+        for n in ("dX", "dWg", "dWu", "dWd"):
+            getattr(b, n).view.fill_(float("nan"))
+        b.backward(pkg, 1, over=over)
+        assert torch.equal(b.get(torch, "H"), first["dG"]) and torch.equal(b.get(torch, over), first["dU"])
+        for n in ("dX", "dWg", "dWu", "dWd"):
+            assert torch.equal(b.get(torch, n), first[n])
+        for n in "GUH":
+            getattr(b, n).view.copy_(kept[n])
     call = pkg.cu32.Cuda_gatedFF.gatedFF_delta
     p = lambda t: t.data_ptr()  # noqa: E731
     for n in ("dX", "dWg", "dWu", "dWd"):
