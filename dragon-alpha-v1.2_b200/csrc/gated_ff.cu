@@ -12,6 +12,7 @@
 #include <atomic>
 
 #include "cu32_host.h"
+#include "gated_thin.h"
 
 namespace dragon {
 namespace {
@@ -654,6 +655,11 @@ int check_dims(int N, int D, int F, int act) {
   return CU32_OK;
 }
 
+long long thin_floats(int N, int D, int F) {
+  const long long up = thin_work_floats(N, F, D, 2), down = thin_work_floats(N, D, F, 1);
+  return up > down ? up : down;
+}
+
 template <class... P>
 bool any_null(const P*... p) { return (... || (p == nullptr)); }
 template <class... P>
@@ -676,7 +682,10 @@ long long cu32_gatedFF_work(int N, int D, int F) {
   const long long c = extra(split_of(PLAIN_TILES, 6, d, f, (N + 31) / 32, any), d * f);       // deltaWg, deltaWu
   const long long e = extra(split_of(PLAIN_TILES, 6, f, d, (N + 31) / 32, any), d * f);       // deltaWd
   const long long m = a > b ? a : b, o = c > e ? c : e;
-  return m > o ? m : o;
+  const long long most = m > o ? m : o;
+  if (N <= ROWS_MAX || N > THIN_MAX_ROWS) return most;
+  const long long thin = thin_floats(N, D, F);
+  return thin > most ? thin : most;
 }
 
 int cu32_gatedFF(const int64_t* s, int length, const float* X, const float* Wg, const float* Wu, const float* Wd, float* G,
@@ -692,6 +701,12 @@ int cu32_gatedFF(const int64_t* s, int length, const float* X, const float* Wg, 
     if (int rc = rows_any<2>(up, st)) return rc;
     const RowsCall down{H, Wd, nullptr, Y, nullptr, nullptr, N, D, F, 0, 1};
     return rows_any<1>(down, st);
+  }
+  if (N <= THIN_MAX_ROWS && work && thin_floats(N, D, F) <= work_floats) {
+    const ThinCall up{X, Wg, Wu, H, G, U, work, N, F, D, act, 0};
+    if (int rc = thin_product(up, st)) return rc;
+    const ThinCall down{H, Wd, nullptr, Y, nullptr, nullptr, work, N, D, F, 0, 1};
+    return thin_product(down, st);
   }
   if (int rc = gated_tiles(X, Wg, Wu, G, U, H, N, D, F, act, st)) return rc;
   return product(s, false, true, H, F, Wd, D, Y, N, D, F, work, work_floats, st);

@@ -1,0 +1,437 @@
+// Products of a few dozen rows with a large weight, FP32-accurate on the tensor cores:
+//   out[n, :] = X[n, :] W   or   act(X[n, :] W0) * (X[n, :] W1),   9 to 128 rows.
+//
+// Every weight is read once for all rows, so the time should be that of reading the weights.  The roles of the operands
+// are therefore exchanged against the general contraction kernel: 128 weight columns are the rows of the tensor core's
+// tile (operand A, MN-major as they lie), the NT rows of X its columns - no tile row is wasted on rows X does not have.
+// Arithmetic as there: hi = what the tensor core makes of an FP32 operand, lo = rounded remainder, written beside it by
+// split warps; lo*hi + hi*lo + hi*hi, at most `kc` k-blocks summed in tensor memory before FP32 registers take over.
+// Up to 64 rows X's lo part lies right behind its hi part, so that one instruction with 2 NT columns forms hi*hi and hi*lo
+// and the weight tile is fetched twice per step instead of three times (the fetches from shared memory bound the step).
+//
+// The work is the list of (128 columns, 32 rows of K) blocks, column block by column block, cut into equal runs, one per
+// SM: no SM idles whatever the width.  A run's sums of a column block go to the caller's scratch and a second kernel
+// adds a column block's runs in order, applies the gate and stores the rows (no atomics: results do not vary).
+#include <atomic>
+
+#include "cu32_host.h"
+#include "gated_thin.h"
+
+namespace dragon {
+namespace {
+
+using namespace ptx;
+
+constexpr int THIN_THREADS = 512, THIN_SPLIT_WARPS = 6, THIN_DRAIN_WARP0 = 8;
+constexpr int ROLE_THIN_LOAD = 13, ROLE_THIN_SPLIT = 14, ROLE_THIN_MMA = 15, ROLE_THIN_DRAIN = 16;
+
+struct ThinParams {
+  CUtensorMap tmW[2];       // [K, M] weights, boxes of 32 x 32 (MN-major slabs)
+  CUtensorMap tmX;          // [N, K], boxes of NT rows x 32 (K-major)
+  float* part;              // [slot][matrix][row][128 columns]
+  int kblocks, items, kc;
+  long long blocks;         // kblocks * items
+  int early;                // the grid may start before the one that writes X has ended
+  int* status;
+};
+
+template <int NT, int MATS>
+struct ThinCfg {
+  static constexpr bool CONCAT = NT <= 64;
+  static constexpr int W_BYTES = MATS * 16384;                    // weight tile of a k-block
+  static constexpr int X_BYTES = NT * 128;
+  static constexpr int RAW = W_BYTES + 2 * X_BYTES;               // weights, X, X lo
+  static constexpr int LO = W_BYTES;                              // lo part of the weights
+  static constexpr int L = MATS == 2 ? 2 : 3;
+  static constexpr int FIT = (225 * 1024 - L * LO) / RAW;
+  static constexpr int R = FIT < 8 ? FIT : 8;
+  static constexpr int SMEM = 1024 + R * RAW + L * LO;
+  static constexpr int DCOLS = CONCAT ? 2 * NT : NT;              // tensor-memory columns per matrix and buffer
+  static constexpr int TMEM_NEED = 2 * MATS * DCOLS;
+  static constexpr int TMEM_COLS = TMEM_NEED <= 64 ? 64 : TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
+  // drain warps: two groups of four; a group takes a matrix, or half the rows of the only one
+  static constexpr bool HALVES = MATS == 1 && NT >= 32;
+  static constexpr int ACC = HALVES ? NT / 2 : NT;
+  static_assert(R >= 2 && TMEM_NEED <= 512 && SMEM <= 227 * 1024 - 512, "thin");
+};
+
+// Run b of `runs`: blocks [first_block(b), first_block(b + 1)).
+__host__ __device__ inline long long first_block(long long b, long long runs, long long blocks) { return b * blocks / runs; }
+// The run that holds block u.
+__host__ __device__ inline int run_of(long long u, long long runs, long long blocks) {
+  return static_cast<int>(((u + 1) * runs + blocks - 1) / blocks - 1);
+}
+
+template <int NT, int MATS>
+__global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_constant__ ThinParams p) {
+  using Cfg = ThinCfg<NT, MATS>;
+  extern __shared__ uint8_t thin_smem[];
+  __shared__ __align__(8) uint64_t bar_tma[8], bar_split[8], bar_empty[8], bar_tmem_full[2], bar_tmem_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t raw = (smem_u32(thin_smem) + 1023u) & ~1023u, lo = raw + Cfg::R * Cfg::RAW;
+  constexpr uint32_t R = Cfg::R, L = Cfg::L;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(smem_u32(&bar_tma[i]), 1);
+      mbar_init(smem_u32(&bar_split[i]), THIN_SPLIT_WARPS);
+      mbar_init(smem_u32(&bar_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_tmem_full[i]), 1);
+      mbar_init(smem_u32(&bar_tmem_empty[i]), 8);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    tmem_alloc<1>(smem_u32(&tmem_slot), Cfg::TMEM_COLS);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const long long u0 = first_block(blockIdx.x, gridDim.x, p.blocks), u1 = first_block(blockIdx.x + 1, gridDim.x, p.blocks);
+  auto give_up = [&](int role, int a, long long b) {
+    abort_flag = 1;
+    atomicCAS(p.status, 0, (role << 24) | ((a & 0xFF) << 16) | static_cast<int>(b & 0xFFFF));
+  };
+
+  if (warp < THIN_DRAIN_WARP0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ---------------------------------------------------------- loads
+      uint32_t s = 0, ph = 0, it = 0;
+      uint32_t held = 0;                   // k-blocks whose X has not been asked for yet
+      bool started = p.early == 0;
+      auto load_x = [&](uint32_t slot, int k) {
+        tma_load_3d(raw + slot * Cfg::RAW + Cfg::W_BYTES, &p.tmX, smem_u32(&bar_tma[slot]), k * 32, 0, 0, 0ull);
+      };
+      auto x_of_held = [&]() {             // weights may be asked for before X exists; X waits for the grid that writes it
+        if (lane == 0) {
+          asm volatile("griddepcontrol.wait;" ::: "memory");
+          for (uint32_t i = 0; i < held; ++i) load_x(i, static_cast<int>((u0 + i) % p.kblocks));
+        }
+        __syncwarp();
+        started = true;
+      };
+      for (long long u = u0; u < u1; ++u, ++it) {
+        if (!started && held == R) x_of_held();
+        if (!mbar_wait(smem_u32(&bar_empty[s]), ph ^ 1u, &abort_flag)) {
+          if (lane == 0) give_up(ROLE_THIN_LOAD, s, it);
+          break;
+        }
+        const int item = static_cast<int>(u / p.kblocks), k = static_cast<int>(u - static_cast<long long>(item) * p.kblocks);
+        if (elect_one()) {
+          const uint32_t bar = smem_u32(&bar_tma[s]), dst = raw + s * Cfg::RAW;
+          mbar_arrive_expect_tx(bar, Cfg::W_BYTES + Cfg::X_BYTES);
+#pragma unroll
+          for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              tma_load_3d(dst + m * 16384 + j * 4096, &p.tmW[m], bar, item * 128 + j * 32, k * 32, 0, 0ull);
+          if (started) load_x(s, k);
+        }
+        __syncwarp();
+        if (!started) ++held;
+        if (++s == R) { s = 0; ph ^= 1u; }
+      }
+      if (!started) x_of_held();
+      if (lane == 0 && abort_flag) {       // copies in flight land before shared memory is released
+        for (uint32_t i = it > R ? it - R : 0u; i < it; ++i) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(smem_u32(&bar_tma[i % R]), (i / R) & 1u) && clock64() - t0 < 20000000LL) {
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------- products
+      constexpr uint32_t ID_WIDE = make_idesc_tf32(128, Cfg::CONCAT ? 2 * NT : NT, true, false);
+      constexpr uint32_t ID_NT = make_idesc_tf32(128, NT, true, false);
+      constexpr uint64_t A_STEP = 1024 >> 4, B_STEP = 32 >> 4;     // 8 rows of K
+      uint32_t s = 0, ph = 0, l = 0, ch = 0;
+      int kk = 0;
+      for (long long u = u0; u < u1; ++u) {
+        const bool seg_end = (u + 1) % p.kblocks == 0 || u + 1 == u1;
+        const bool first = kk == 0;
+        const bool last = ++kk == p.kc || seg_end;
+        if (last) kk = 0;
+        if (!mbar_wait(smem_u32(&bar_split[s]), ph, &abort_flag)) {
+          if (lane == 0) give_up(ROLE_THIN_MMA, s, u - u0);
+          break;
+        }
+        const uint32_t buf = ch & 1u;
+        if (first && !mbar_wait(smem_u32(&bar_tmem_empty[buf]), ((ch >> 1) & 1u) ^ 1u, &abort_flag)) {
+          if (lane == 0) give_up(ROLE_THIN_MMA, 50 + buf, u - u0);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t x = raw + s * Cfg::RAW + Cfg::W_BYTES;
+        if (elect_one()) {
+          const uint64_t bx = make_smem_desc(x, 16u, 1024u, SMEM_LAYOUT_SW128);
+          const uint64_t bxl = make_smem_desc(x + Cfg::X_BYTES, 16u, 1024u, SMEM_LAYOUT_SW128);
+          const uint32_t fresh = first ? 0u : 1u;
+#pragma unroll
+          for (int m = 0; m < MATS; ++m) {
+            const uint64_t a_hi = make_smem_desc(raw + s * Cfg::RAW + m * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
+            const uint64_t a_lo = make_smem_desc(lo + l * Cfg::LO + m * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
+            const uint32_t d = tmem + (buf * MATS + m) * Cfg::DCOLS;
+            if (Cfg::CONCAT) {
+              // columns [0, NT): hi*hi; columns [NT, 2 NT): hi*lo, then lo*hi
+#pragma unroll
+              for (int j = 0; j < 4; ++j) umma_tf32<1>(d, a_hi + j * A_STEP, bx + j * B_STEP, ID_WIDE, j == 0 ? fresh : 1u);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) umma_tf32<1>(d + NT, a_lo + j * A_STEP, bx + j * B_STEP, ID_NT, 1u);
+            } else {
+              // the small products first, while the truncating accumulator is small
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                umma_tf32<1>(d, a_lo + j * A_STEP, bx + j * B_STEP, ID_NT, j == 0 ? fresh : 1u);
+                umma_tf32<1>(d, a_hi + j * A_STEP, bxl + j * B_STEP, ID_NT, 1u);
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) umma_tf32<1>(d, a_hi + j * A_STEP, bx + j * B_STEP, ID_NT, 1u);
+            }
+          }
+          umma_commit<1>(smem_u32(&bar_empty[s]));
+          if (last) umma_commit<1>(smem_u32(&bar_tmem_full[buf]));
+        }
+        __syncwarp();
+        if (++s == R) { s = 0; ph ^= 1u; }
+        if (++l == L) l = 0;
+        if (last) ++ch;
+      }
+    } else {
+      // ---------------------------------------------------------- split
+      const int st = (warp - 2) * 32 + lane;
+      constexpr int NST = THIN_SPLIT_WARPS * 32;
+      constexpr int VW = Cfg::W_BYTES / 16, VX = Cfg::X_BYTES / 16;
+      static_assert(VW % 32 == 0 && VX % 32 == 0, "a warp's 32 vectors are 512 contiguous bytes");
+      uint32_t s = 0, ph = 0, l = 0, sp = 0, php = 0, it = 0;
+      for (long long u = u0; u < u1; ++u, ++it) {
+        if (!mbar_wait(smem_u32(&bar_tma[s]), ph, &abort_flag)) {
+          if (lane == 0) give_up(ROLE_THIN_SPLIT, s, it);
+          break;
+        }
+        if (L != R && it >= L) {           // the lo slot is free once the products of k-block it - L are done
+          if (!mbar_wait(smem_u32(&bar_empty[sp]), php, &abort_flag)) {
+            if (lane == 0) give_up(ROLE_THIN_SPLIT, 100 + sp, it);
+            break;
+          }
+        }
+        const uint32_t from = raw + s * Cfg::RAW, to_w = lo + l * Cfg::LO;
+        auto lo_of = [](float4 x) {
+          return make_float4(rn_tf32(x.x - trunc_tf32(x.x)), rn_tf32(x.y - trunc_tf32(x.y)), rn_tf32(x.z - trunc_tf32(x.z)),
+                             rn_tf32(x.w - trunc_tf32(x.w)));
+        };
+        constexpr int PER = (VW + NST - 1) / NST, G = 4;
+#pragma unroll
+        for (int b = 0; b < PER; b += G) {
+          float4 x[G];
+#pragma unroll
+          for (int i = 0; i < G; ++i) {
+            const int v = st + (b + i) * NST;
+            if (b + i < PER && v < VW) x[i] = lds2x64(from + (v - lane) * 16, lane);
+          }
+#pragma unroll
+          for (int i = 0; i < G; ++i) {
+            const int v = st + (b + i) * NST;
+            if (b + i < PER && v < VW) sts2x64(to_w + (v - lane) * 16, lane, lo_of(x[i]));
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < (VX + NST - 1) / NST; ++b) {
+          const int v = st + b * NST;
+          if (v < VX) {
+            const float4 x = lds2x64(from + Cfg::W_BYTES + (v - lane) * 16, lane);
+            sts2x64(from + Cfg::W_BYTES + Cfg::X_BYTES + (v - lane) * 16, lane, lo_of(x));
+          }
+        }
+        fence_proxy_async_smem();          // the tensor core reads these through the async proxy
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_split[s]));
+        if (++s == R) { s = 0; ph ^= 1u; }
+        if (++l == L) l = 0;
+        if (it + 1 > L && ++sp == R) { sp = 0; php ^= 1u; }      // (sp, php): k-block it + 1 - L
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ drain: tensor memory -> registers -> scratch
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const int q = warp & 3, h = (warp - THIN_DRAIN_WARP0) >> 2;
+    const int m = MATS == 2 ? h : 0, t0 = Cfg::HALVES ? h * Cfg::ACC : 0;
+    const bool works = MATS == 2 || Cfg::HALVES || h == 0;
+    uint32_t ch = 0;
+    bool alive = true;
+    for (long long u = u0; alive && u < u1;) {
+      const int item = static_cast<int>(u / p.kblocks);
+      const long long end = static_cast<long long>(item + 1) * p.kblocks < u1 ? static_cast<long long>(item + 1) * p.kblocks : u1;
+      float acc[Cfg::ACC];
+#pragma unroll
+      for (int t = 0; t < Cfg::ACC; ++t) acc[t] = 0.0f;
+      for (; u < end; u += p.kc, ++ch) {
+        const uint32_t buf = ch & 1u;
+        if (!mbar_wait(smem_u32(&bar_tmem_full[buf]), (ch >> 1) & 1u, &abort_flag)) {
+          if (lane == 0) give_up(ROLE_THIN_DRAIN, buf, u - u0);
+          alive = false;
+          break;
+        }
+        tc_fence_after();
+        if (works) {
+          const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + (buf * MATS + m) * Cfg::DCOLS + t0;
+#pragma unroll
+          for (int t = 0; t < Cfg::ACC; t += 16) {
+            float big[16], small[16];
+            tmem_ld_32x16(at + t, big);
+            if (Cfg::CONCAT) tmem_ld_32x16(at + NT + t, small);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[t + j] += Cfg::CONCAT ? big[j] + small[j] : big[j];
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[buf]));
+      }
+      u = end;
+      if (alive && works) {
+        // slot: run + item, which grows from one segment of the list to the next
+        float* out = p.part + ((static_cast<long long>(blockIdx.x) + item) * MATS + m) * (NT * 128) + t0 * 128 + q * 32 + lane;
+#pragma unroll
+        for (int t = 0; t < Cfg::ACC; ++t) out[t * 128] = acc[t];
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
+  }
+}
+
+// Sums of a column block's runs in order, gate, rows out.  One 16-byte vector of a row per thread.
+struct ThinSumParams {
+  const float* part;
+  float* out; float* G; float* U;
+  int N, M, act, kblocks, runs;
+  long long blocks;
+};
+template <int NT, int MATS>
+__global__ void __launch_bounds__(256) thin_sum_kernel(const __grid_constant__ ThinSumParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int vecs = p.M / 4;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < static_cast<long long>(p.N) * vecs;
+       i += static_cast<long long>(gridDim.x) * 256) {
+    const int n = static_cast<int>(i / vecs), v = static_cast<int>(i - static_cast<long long>(n) * vecs);
+    const int item = v >> 5;
+    const long long first = static_cast<long long>(item) * p.kblocks;
+    const int b0 = run_of(first, p.runs, p.blocks), b1 = run_of(first + p.kblocks - 1, p.runs, p.blocks);
+    float s[MATS * 4];
+#pragma unroll
+    for (int k = 0; k < MATS * 4; ++k) s[k] = 0.0f;
+    for (int b = b0; b <= b1; ++b) {
+#pragma unroll
+      for (int m = 0; m < MATS; ++m) {
+        const float4 x = *reinterpret_cast<const float4*>(
+            p.part + (((static_cast<long long>(b) + item) * MATS + m) * NT + n) * 128 + (v & 31) * 4);
+        s[m * 4] += x.x; s[m * 4 + 1] += x.y; s[m * 4 + 2] += x.z; s[m * 4 + 3] += x.w;
+      }
+    }
+    const long long at = static_cast<long long>(n) * p.M + v * 4;
+    if constexpr (MATS == 2) {
+      if (p.G != nullptr) {
+        *reinterpret_cast<float4*>(p.G + at) = make_float4(s[0], s[1], s[2], s[3]);
+        *reinterpret_cast<float4*>(p.U + at) = make_float4(s[4], s[5], s[6], s[7]);
+      }
+      gated_forward<4>(p.act, s);
+    }
+    *reinterpret_cast<float4*>(p.out + at) = make_float4(s[0], s[1], s[2], s[3]);
+  }
+}
+
+int runs_of(long long blocks) {
+  // a run shorter than four k-blocks costs more in its sums than it saves
+  const long long most = device_sm_count(), want = (blocks + 3) / 4;
+  return static_cast<int>(want < most ? want : most);
+}
+
+template <int NT, int MATS>
+int thin_launch(const ThinCall& c, cudaStream_t st) {
+  using Cfg = ThinCfg<NT, MATS>;
+  auto kernel = thin_kernel<NT, MATS>;
+  static std::atomic<int> ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (!ready[dev & 63].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    ready[dev & 63].store(1, std::memory_order_release);
+  }
+  ThinParams p;
+  std::memset(&p, 0, sizeof(p));
+  const uint64_t n = c.N, k = c.K, m = c.M;
+  if (int rc = make_map3(&p.tmW[0], c.W0, m, k, 1, m, m * k, 32, 32, true)) return rc;
+  if (MATS == 2)
+    if (int rc = make_map3(&p.tmW[1], c.W1, m, k, 1, m, m * k, 32, 32, true)) return rc;
+  if (int rc = make_map3(&p.tmX, c.X, k, n, 1, k, k * n, 32, NT, false)) return rc;
+  p.part = c.work;
+  p.kblocks = (c.K + 31) / 32;
+  p.items = (c.M + 127) / 128;
+  p.blocks = static_cast<long long>(p.kblocks) * p.items;
+  p.kc = tuned_kc();
+  p.early = c.early;
+  p.status = status_word_ptr(&e);
+  if (!p.status) return static_cast<int>(e);
+  const int runs = runs_of(p.blocks);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(runs, 1, 1);
+  cfg.blockDim = dim3(THIN_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = c.early ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  ThinSumParams q{};
+  q.part = c.work; q.out = c.out; q.G = c.G; q.U = c.U;
+  q.N = c.N; q.M = c.M; q.act = c.act; q.kblocks = p.kblocks; q.runs = runs; q.blocks = p.blocks;
+  const long long vecs = static_cast<long long>(c.N) * (c.M / 4);
+  long long grid = (vecs + 255) / 256;
+  if (grid > 8LL * device_sm_count()) grid = 8LL * device_sm_count();
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, thin_sum_kernel<NT, MATS>, q));
+}
+
+int thin_rows(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; }
+
+}  // namespace
+
+long long thin_work_floats(int N, int M, int K, int mats) {
+  const long long items = (M + 127) / 128, blocks = items * ((K + 31) / 32);
+  return (runs_of(blocks) + items - 1) * mats * thin_rows(N) * 128;
+}
+
+int thin_product(const ThinCall& c, cudaStream_t st) {
+  if (!load_driver_entry_points()) return CU32_E_DRIVER;
+  const bool gated = c.W1 != nullptr;
+  switch (thin_rows(c.N)) {
+    case 16: return gated ? thin_launch<16, 2>(c, st) : thin_launch<16, 1>(c, st);
+    case 32: return gated ? thin_launch<32, 2>(c, st) : thin_launch<32, 1>(c, st);
+    case 64: return gated ? thin_launch<64, 2>(c, st) : thin_launch<64, 1>(c, st);
+    default: return gated ? thin_launch<128, 2>(c, st) : thin_launch<128, 1>(c, st);
+  }
+}
+
+}  // namespace dragon

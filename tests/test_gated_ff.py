@@ -153,9 +153,10 @@ def test_gated_ff_refusals(pkg):
 
 # ---------------------------------------------------------------------------------------------------- on the GPU
 SHAPES = [
-    # N, D, F: few rows (one kernel per row count), then tiles with every kind of tail
+    # N, D, F: up to 8 rows, up to 128 rows (both: one kernel per power of two), tiles; with every kind of tail
     (1, 4, 4), (1, 64, 132), (2, 36, 260), (3, 516, 64), (4, 128, 128), (5, 132, 1028), (8, 1028, 516), (9, 68, 36),
-    (16, 260, 2052), (17, 4, 4), (17, 36, 68), (33, 128, 260), (128, 64, 64), (130, 260, 516), (257, 516, 132),
+    (16, 260, 2052), (17, 4, 4), (17, 36, 68), (33, 128, 260), (128, 64, 64), (10, 4, 4), (24, 36, 4100),
+    (64, 1028, 516), (65, 260, 260), (100, 2052, 132), (130, 260, 516), (257, 516, 132),
     (520, 132, 1028),
 ]
 
@@ -192,21 +193,22 @@ def test_gated_ff_on_every_tile(pkg, cuda, tile):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [(1, 2052, 132), (7, 68, 516), (200, 516, 260)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 2052, 132), (7, 68, 516), (12, 516, 132), (50, 132, 1028), (200, 516, 260)], ids=str)
 def test_serving_gives_the_bits_of_training_and_repeats(pkg, cuda, shape):
     torch = cuda
     b = Block(torch, *shape, seed=3)
-    b.forward(pkg, 2, save=True)
+    work = torch.full((pkg.cu32.Cuda_gatedFF.work(*shape) + 4,), float("nan"), device="cuda")
+    b.forward(pkg, 2, save=True, work=work)
     H, Y = b.get(torch, "H"), b.get(torch, "Y")
     for save in (False, True, False):
         b.H.view.fill_(float("nan"))
         b.Y.view.fill_(float("nan"))
-        b.forward(pkg, 2, save=save)
+        b.forward(pkg, 2, save=save, work=work)
         assert torch.equal(b.get(torch, "H"), H) and torch.equal(b.get(torch, "Y"), Y)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [(1, 8228, 68), (33, 8228, 68), (40, 64, 20004)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 8228, 68), (33, 8228, 68), (40, 64, 20004), (130, 8228, 68), (150, 64, 20004)], ids=str)
 def test_long_reductions(pkg, cuda, shape):
     """A width beyond the interval after which plain products flush their sums, and a long hidden axis cut into slices."""
     torch = cuda
@@ -284,6 +286,22 @@ def test_far_pre_activations(pkg, cuda, act, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [20, 128])
+def test_without_scratch(pkg, cuda, rows):
+    """No scratch, or too little: the same call by another path, nothing written beyond what was given."""
+    torch = cuda
+    b = Block(torch, rows, 516, 772, seed=10)
+    need = pkg.cu32.Cuda_gatedFF.work(rows, 516, 772)
+    for room in (0, need // 2 // 4 * 4, need):
+        work = torch.full((need + 64,), 7.0, device="cuda")
+        b.forward(pkg, 0, work=work[:room] if room else None)
+        check_forward(torch, b, 0)
+        b.backward(pkg, 0, work=work[:room] if room else None)
+        check_backward(torch, b, 0, b.get(torch, "G"), b.get(torch, "U"))
+        assert (work[room:] == 7.0).all()
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences(pkg, cuda):
     """deltaX and the weight gradients against central differences of sum(Y deltaY) taken in 64 bits: the formula itself."""
     torch = cuda
@@ -309,19 +327,20 @@ def test_gradients_against_differences(pkg, cuda):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [2, 64])
+@pytest.mark.parametrize("rows", [2, 64, 200])
 def test_on_a_stream_of_its_own_and_in_a_graph(pkg, cuda, rows):
     """The calls run on streams[0] alone; captured once, replayed with new inputs, forward and gradients."""
     torch = cuda
     b = Block(torch, rows, 132, 260, seed=8)
-    b.forward(pkg, 0)          # first use outside the capture
-    b.backward(pkg, 0)
+    work = torch.empty(pkg.cu32.Cuda_gatedFF.work(rows, 132, 260) + 4, device="cuda")
+    b.forward(pkg, 0, work=work)          # first use outside the capture
+    b.backward(pkg, 0, work=work)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=s):
-        b.forward(pkg, 0)
-        b.backward(pkg, 0)
+        b.forward(pkg, 0, work=work)
+        b.backward(pkg, 0, work=work)
     b.X.mul_(0.5).add_(0.25)
     b.dY.mul_(-1.5)
     graph.replay()
@@ -333,9 +352,9 @@ def test_on_a_stream_of_its_own_and_in_a_graph(pkg, cuda, rows):
 
 @pytest.mark.gpu
 def test_two_streams_at_once(pkg, cuda):
-    """Two blocks on two streams, each with scratch of its own."""
+    """Blocks on streams of their own, each with scratch of its own."""
     torch = cuda
-    blocks = [Block(torch, n, 260, 1028, seed=50 + n) for n in (5, 300)]
+    blocks = [Block(torch, n, 260, 1028, seed=50 + n) for n in (5, 30, 300)]
     works = [torch.empty(pkg.cu32.Cuda_gatedFF.work(b.N, b.D, b.F) + 4, device="cuda") for b in blocks]
     streams = [torch.cuda.Stream() for _ in blocks]
     torch.cuda.synchronize()
@@ -354,12 +373,13 @@ def test_two_streams_at_once(pkg, cuda):
 def test_rows_do_not_depend_on_their_company(pkg, cuda):
     """A NaN in one row stays in that row, forward and in deltaX."""
     torch = cuda
-    for rows in (4, 40):
+    for rows in (4, 40, 140):
         b = Block(torch, rows, 68, 132, seed=9)
-        b.forward(pkg, 0)
+        work = torch.empty(pkg.cu32.Cuda_gatedFF.work(rows, 68, 132) + 4, device="cuda")
+        b.forward(pkg, 0, work=work)
         clean = b.get(torch, "Y")
         b.X[2, 5] = float("nan")
-        b.forward(pkg, 0)
+        b.forward(pkg, 0, work=work)
         Y = b.get(torch, "Y")
         assert torch.isnan(Y[2]).all()
         others = [i for i in range(rows) if i != 2]
