@@ -22,7 +22,7 @@ namespace {
 
 using namespace ptx;
 
-constexpr int THIN_THREADS = 512, THIN_SPLIT_WARPS = 6, THIN_DRAIN_WARP0 = 8;
+constexpr int THIN_THREADS = 512;
 constexpr int ROLE_THIN_LOAD = 13, ROLE_THIN_SPLIT = 14, ROLE_THIN_MMA = 15, ROLE_THIN_DRAIN = 16;
 
 struct ThinParams {
@@ -49,9 +49,15 @@ struct ThinCfg {
   static constexpr int DCOLS = CONCAT ? 2 * NT : NT;              // tensor-memory columns per matrix and buffer
   static constexpr int TMEM_NEED = 2 * MATS * DCOLS;
   static constexpr int TMEM_COLS = TMEM_NEED <= 64 ? 64 : TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
-  // drain warps: two groups of four; a group takes a matrix, or half the rows of the only one
-  static constexpr bool HALVES = MATS == 1 && NT >= 32;
-  static constexpr int ACC = HALVES ? NT / 2 : NT;
+  // Drain warps: four hold all sums of their 32 columns as long as those are 128 at most; the other ten of the sixteen
+  // warps split (with six the split took longer than the weights' way from memory: 140 us for 16 rows of 4096 / 10924).
+  // 128 rows of two matrices: eight drain warps, a matrix each half.
+  static constexpr int DRAIN_WARPS = MATS * NT <= 128 ? 4 : 8;
+  static constexpr int DRAIN_WARP0 = 16 - DRAIN_WARPS, SPLIT_WARPS = DRAIN_WARP0 - 2;
+  static constexpr int MINE = DRAIN_WARPS == 4 ? MATS : 1;        // matrices per drain warp
+  // registers after reallocation, per thread: 64 K in all
+  static constexpr int REGS_MOVERS = DRAIN_WARPS == 4 ? 96 : 72, REGS_DRAINERS = DRAIN_WARPS == 4 ? 216 : 184;
+  static_assert(REGS_MOVERS * DRAIN_WARP0 * 32 + REGS_DRAINERS * DRAIN_WARPS * 32 <= 65536, "registers");
   static_assert(R >= 2 && TMEM_NEED <= 512 && SMEM <= 227 * 1024 - 512, "thin");
 };
 
@@ -76,12 +82,12 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
     abort_flag = 0;
     for (int i = 0; i < 8; ++i) {
       mbar_init(smem_u32(&bar_tma[i]), 1);
-      mbar_init(smem_u32(&bar_split[i]), THIN_SPLIT_WARPS);
+      mbar_init(smem_u32(&bar_split[i]), Cfg::SPLIT_WARPS);
       mbar_init(smem_u32(&bar_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bar_tmem_full[i]), 1);
-      mbar_init(smem_u32(&bar_tmem_empty[i]), 8);
+      mbar_init(smem_u32(&bar_tmem_empty[i]), Cfg::DRAIN_WARPS);
     }
     fence_mbar_init();
   }
@@ -94,14 +100,18 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const long long u0 = first_block(blockIdx.x, gridDim.x, p.blocks), u1 = first_block(blockIdx.x + 1, gridDim.x, p.blocks);
-  auto give_up = [&](int role, int a, long long b) {
+  // this run: `count` blocks from k-block k_first of column block item_first on (every role carries (item, k) along: a
+  // division per block would cost the issuing thread more than the products it issues)
+  const long long u0 = first_block(blockIdx.x, gridDim.x, p.blocks);
+  const int count = static_cast<int>(first_block(blockIdx.x + 1, gridDim.x, p.blocks) - u0);
+  const int item_first = static_cast<int>(u0 / p.kblocks), k_first = static_cast<int>(u0 - static_cast<long long>(item_first) * p.kblocks);
+  auto give_up = [&](int role, int a, int b) {
     abort_flag = 1;
-    atomicCAS(p.status, 0, (role << 24) | ((a & 0xFF) << 16) | static_cast<int>(b & 0xFFFF));
+    atomicCAS(p.status, 0, (role << 24) | ((a & 0xFF) << 16) | (b & 0xFFFF));
   };
 
-  if (warp < THIN_DRAIN_WARP0) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp < Cfg::DRAIN_WARP0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_MOVERS));
     if (warp == 0) {
       // ---------------------------------------------------------- loads
       uint32_t s = 0, ph = 0, it = 0;
@@ -113,18 +123,18 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
       auto x_of_held = [&]() {             // weights may be asked for before X exists; X waits for the grid that writes it
         if (lane == 0) {
           asm volatile("griddepcontrol.wait;" ::: "memory");
-          for (uint32_t i = 0; i < held; ++i) load_x(i, static_cast<int>((u0 + i) % p.kblocks));
+          for (uint32_t i = 0; i < held; ++i) load_x(i, (k_first + static_cast<int>(i)) % p.kblocks);
         }
         __syncwarp();
         started = true;
       };
-      for (long long u = u0; u < u1; ++u, ++it) {
+      int item = item_first, k = k_first;
+      for (; it < static_cast<uint32_t>(count); ++it) {
         if (!started && held == R) x_of_held();
         if (!mbar_wait(smem_u32(&bar_empty[s]), ph ^ 1u, &abort_flag)) {
           if (lane == 0) give_up(ROLE_THIN_LOAD, s, it);
           break;
         }
-        const int item = static_cast<int>(u / p.kblocks), k = static_cast<int>(u - static_cast<long long>(item) * p.kblocks);
         if (elect_one()) {
           const uint32_t bar = smem_u32(&bar_tma[s]), dst = raw + s * Cfg::RAW;
           mbar_arrive_expect_tx(bar, Cfg::W_BYTES + Cfg::X_BYTES);
@@ -137,6 +147,7 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
         }
         __syncwarp();
         if (!started) ++held;
+        if (++k == p.kblocks) { k = 0; ++item; }
         if (++s == R) { s = 0; ph ^= 1u; }
       }
       if (!started) x_of_held();
@@ -153,19 +164,20 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
       constexpr uint32_t ID_NT = make_idesc_tf32(128, NT, true, false);
       constexpr uint64_t A_STEP = 1024 >> 4, B_STEP = 32 >> 4;     // 8 rows of K
       uint32_t s = 0, ph = 0, l = 0, ch = 0;
-      int kk = 0;
-      for (long long u = u0; u < u1; ++u) {
-        const bool seg_end = (u + 1) % p.kblocks == 0 || u + 1 == u1;
+      int kk = 0, k = k_first;
+      for (int i = 0; i < count; ++i) {
+        if (++k == p.kblocks) k = 0;
+        const bool seg_end = k == 0 || i + 1 == count;
         const bool first = kk == 0;
         const bool last = ++kk == p.kc || seg_end;
         if (last) kk = 0;
         if (!mbar_wait(smem_u32(&bar_split[s]), ph, &abort_flag)) {
-          if (lane == 0) give_up(ROLE_THIN_MMA, s, u - u0);
+          if (lane == 0) give_up(ROLE_THIN_MMA, s, i);
           break;
         }
         const uint32_t buf = ch & 1u;
         if (first && !mbar_wait(smem_u32(&bar_tmem_empty[buf]), ((ch >> 1) & 1u) ^ 1u, &abort_flag)) {
-          if (lane == 0) give_up(ROLE_THIN_MMA, 50 + buf, u - u0);
+          if (lane == 0) give_up(ROLE_THIN_MMA, 50 + buf, i);
           break;
         }
         tc_fence_after();
@@ -207,11 +219,11 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
     } else {
       // ---------------------------------------------------------- split
       const int st = (warp - 2) * 32 + lane;
-      constexpr int NST = THIN_SPLIT_WARPS * 32;
+      constexpr int NST = Cfg::SPLIT_WARPS * 32;
       constexpr int VW = Cfg::W_BYTES / 16, VX = Cfg::X_BYTES / 16;
       static_assert(VW % 32 == 0 && VX % 32 == 0, "a warp's 32 vectors are 512 contiguous bytes");
       uint32_t s = 0, ph = 0, l = 0, sp = 0, php = 0, it = 0;
-      for (long long u = u0; u < u1; ++u, ++it) {
+      for (; it < static_cast<uint32_t>(count); ++it) {
         if (!mbar_wait(smem_u32(&bar_tma[s]), ph, &abort_flag)) {
           if (lane == 0) give_up(ROLE_THIN_SPLIT, s, it);
           break;
@@ -260,48 +272,52 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
     }
   } else {
     // ------------------------------------------------------------ drain: tensor memory -> registers -> scratch
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-    const int q = warp & 3, h = (warp - THIN_DRAIN_WARP0) >> 2;
-    const int m = MATS == 2 ? h : 0, t0 = Cfg::HALVES ? h * Cfg::ACC : 0;
-    const bool works = MATS == 2 || Cfg::HALVES || h == 0;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_DRAINERS));
+    constexpr int MINE = Cfg::MINE;
+    const int q = warp & 3, m0 = MINE == MATS ? 0 : (warp - Cfg::DRAIN_WARP0) >> 2;
     uint32_t ch = 0;
     bool alive = true;
-    for (long long u = u0; alive && u < u1;) {
-      const int item = static_cast<int>(u / p.kblocks);
-      const long long end = static_cast<long long>(item + 1) * p.kblocks < u1 ? static_cast<long long>(item + 1) * p.kblocks : u1;
-      float acc[Cfg::ACC];
+    int item = item_first, k = k_first;
+    for (int i = 0; alive && i < count; ++item, k = 0) {
+      const int end = min(i + p.kblocks - k, count);
+      float acc[MINE][NT];
 #pragma unroll
-      for (int t = 0; t < Cfg::ACC; ++t) acc[t] = 0.0f;
-      for (; u < end; u += p.kc, ++ch) {
+      for (int m = 0; m < MINE; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[m][t] = 0.0f;
+      for (; i < end; i += p.kc, ++ch) {
         const uint32_t buf = ch & 1u;
         if (!mbar_wait(smem_u32(&bar_tmem_full[buf]), (ch >> 1) & 1u, &abort_flag)) {
-          if (lane == 0) give_up(ROLE_THIN_DRAIN, buf, u - u0);
+          if (lane == 0) give_up(ROLE_THIN_DRAIN, buf, i);
           alive = false;
           break;
         }
         tc_fence_after();
-        if (works) {
-          const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + (buf * MATS + m) * Cfg::DCOLS + t0;
 #pragma unroll
-          for (int t = 0; t < Cfg::ACC; t += 16) {
+        for (int m = 0; m < MINE; ++m) {
+          const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + (buf * MATS + m0 + m) * Cfg::DCOLS;
+#pragma unroll
+          for (int t = 0; t < NT; t += 16) {
             float big[16], small[16];
             tmem_ld_32x16(at + t, big);
             if (Cfg::CONCAT) tmem_ld_32x16(at + NT + t, small);
             tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) acc[t + j] += Cfg::CONCAT ? big[j] + small[j] : big[j];
+            for (int j = 0; j < 16; ++j) acc[m][t + j] += Cfg::CONCAT ? big[j] + small[j] : big[j];
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[buf]));
       }
-      u = end;
-      if (alive && works) {
+      i = end;
+      if (alive) {
         // slot: run + item, which grows from one segment of the list to the next
-        float* out = p.part + ((static_cast<long long>(blockIdx.x) + item) * MATS + m) * (NT * 128) + t0 * 128 + q * 32 + lane;
+        float* out = p.part + ((static_cast<long long>(blockIdx.x) + item) * MATS + m0) * (NT * 128) + q * 32 + lane;
 #pragma unroll
-        for (int t = 0; t < Cfg::ACC; ++t) out[t * 128] = acc[t];
+        for (int m = 0; m < MINE; ++m)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) out[(m * NT + t) * 128] = acc[m][t];
       }
     }
   }
