@@ -1,7 +1,8 @@
 // Products of a few dozen rows with a large weight, FP32-accurate on the tensor cores:
 //   out[n, :] = X[n, :] W   or   act(X[n, :] W0) * (X[n, :] W1),   9 to 128 rows.
 //
-// Every weight is read once for all rows, so the time should be that of reading the weights.  The roles of the operands
+// Every weight is read once for all rows, so the time should be that of reading the weights (with the general kernel it was
+// three times that: 315 us for 16 rows of a 4096 / 10924 block, 537 MB).  The roles of the operands
 // are therefore exchanged against the general contraction kernel: 128 weight columns are the rows of the tensor core's
 // tile (operand A, MN-major as they lie), the NT rows of X its columns - no tile row is wasted on rows X does not have.
 // Arithmetic as there: hi = what the tensor core makes of an FP32 operand, lo = rounded remainder, written beside it by
@@ -9,9 +10,11 @@
 // Up to 64 rows X's lo part lies right behind its hi part, so that one instruction with 2 NT columns forms hi*hi and hi*lo
 // and the weight tile is fetched twice per step instead of three times (the fetches from shared memory bound the step).
 //
-// The work is the list of (128 columns, 32 rows of K) blocks, column block by column block, cut into equal runs, one per
-// SM: no SM idles whatever the width.  A run's sums of a column block go to the caller's scratch and a second kernel
-// adds a column block's runs in order, applies the gate and stores the rows (no atomics: results do not vary).
+// The work is cut into slices, 128 columns by a share of K, so many that whole rounds of them occupy every SM, and
+// numbered with the column block running fastest: what the SMs read at one time are neighbouring columns of the same
+// rows.  (Equal runs of a list ordered column block by column block balance better, but read scattered 512-byte pieces:
+// 4 TB/s, and asking for them earlier made it slower still.)  A slice's sums go to the caller's scratch and a second kernel
+// adds a column block's slices in order, applies the gate and stores the rows (no atomics: results do not vary).
 #include <atomic>
 
 #include "cu32_host.h"
@@ -28,49 +31,48 @@ constexpr int ROLE_THIN_LOAD = 13, ROLE_THIN_SPLIT = 14, ROLE_THIN_MMA = 15, ROL
 struct ThinParams {
   CUtensorMap tmW[2];       // [K, M] weights, boxes of 32 x 32 (MN-major slabs)
   CUtensorMap tmX;          // [N, K], boxes of NT rows x 32 (K-major)
-  float* part;              // [slot][matrix][row][128 columns]
-  int kblocks, items, kc;
-  long long blocks;         // kblocks * items
+  float* part;              // [slice][row][128 columns]
+  int stages, items, slices, chunk;    // slice id: share of K * items + item; items: column blocks, matrix by matrix;
+                                       // K in stages of 32 KS rows, `chunk` of them summed in tensor memory
+  int blocks;                          // column blocks of a matrix
   int early;                // the grid may start before the one that writes X has ended
   int* status;
 };
 
-template <int NT, int MATS>
+template <int NT>
 struct ThinCfg {
   static constexpr bool CONCAT = NT <= 64;
-  static constexpr int W_BYTES = MATS * 16384;                    // weight tile of a k-block
-  static constexpr int X_BYTES = NT * 128;
-  static constexpr int RAW = W_BYTES + 2 * X_BYTES;               // weights, X, X lo
+  // Rows of 32 per stage of the ring.  What a stage costs whatever its size - the issuing thread's waits and commits, the
+  // split's fence - is 700 cycles, the time 16 KB take from memory: two rows of blocks share it where the ring allows.
+  static constexpr int KS = NT <= 32 ? 2 : 1;
+  static constexpr int W_BYTES = KS * 16384;                      // weights of a stage
+  static constexpr int X_BYTES = NT * 128;                        // X of 32 rows of K; its lo part behind it
+  static constexpr int RAW = W_BYTES + KS * 2 * X_BYTES;
   static constexpr int LO = W_BYTES;                              // lo part of the weights
-  static constexpr int L = MATS == 2 ? 2 : 3;
+  // A lo slot is held from the split until the products that read it are seen to be done.
+  static constexpr int L = KS == 2 ? 2 : 3;
   static constexpr int FIT = (225 * 1024 - L * LO) / RAW;
   static constexpr int R = FIT < 8 ? FIT : 8;
   static constexpr int SMEM = 1024 + R * RAW + L * LO;
-  static constexpr int DCOLS = CONCAT ? 2 * NT : NT;              // tensor-memory columns per matrix and buffer
-  static constexpr int TMEM_NEED = 2 * MATS * DCOLS;
-  static constexpr int TMEM_COLS = TMEM_NEED <= 64 ? 64 : TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
-  // Drain warps: four hold all sums of their 32 columns as long as those are 128 at most; the other ten of the sixteen
-  // warps split (with six the split took longer than the weights' way from memory: 140 us for 16 rows of 4096 / 10924).
-  // 128 rows of two matrices: eight drain warps, a matrix each half.
-  static constexpr int DRAIN_WARPS = MATS * NT <= 128 ? 4 : 8;
-  static constexpr int DRAIN_WARP0 = 16 - DRAIN_WARPS, SPLIT_WARPS = DRAIN_WARP0 - 2;
-  static constexpr int MINE = DRAIN_WARPS == 4 ? MATS : 1;        // matrices per drain warp
-  // registers after reallocation, per thread: 64 K in all
-  static constexpr int REGS_MOVERS = DRAIN_WARPS == 4 ? 96 : 72, REGS_DRAINERS = DRAIN_WARPS == 4 ? 216 : 184;
+  static constexpr int DCOLS = CONCAT ? 2 * NT : NT;              // tensor-memory columns per buffer
+  static constexpr int TMEM_COLS = 2 * DCOLS <= 64 ? 64 : 2 * DCOLS <= 128 ? 128 : 256;
+  // Four drain warps hold all sums of their 32 columns.  Ten of the sixteen warps split: all on one stage, or, where a
+  // stage is small, in groups of five that take the stages in turn (a split is mostly latency).
+  static constexpr int DRAIN_WARPS = 4, DRAIN_WARP0 = 16 - DRAIN_WARPS, GROUPS = KS == 2 ? 1 : 2,
+                       SPLIT_WARPS = (DRAIN_WARP0 - 2) / GROUPS;
+  static constexpr int REGS_MOVERS = 96, REGS_DRAINERS = 216;     // per thread after reallocation, 64 K in all
   static_assert(REGS_MOVERS * DRAIN_WARP0 * 32 + REGS_DRAINERS * DRAIN_WARPS * 32 <= 65536, "registers");
-  static_assert(R >= 2 && TMEM_NEED <= 512 && SMEM <= 227 * 1024 - 512, "thin");
+  static_assert(R >= L && 2 * DCOLS <= 256 && SMEM <= 227 * 1024 - 512, "thin");
 };
 
-// Run b of `runs`: blocks [first_block(b), first_block(b + 1)).
-__host__ __device__ inline long long first_block(long long b, long long runs, long long blocks) { return b * blocks / runs; }
-// The run that holds block u.
-__host__ __device__ inline int run_of(long long u, long long runs, long long blocks) {
-  return static_cast<int>(((u + 1) * runs + blocks - 1) / blocks - 1);
+// First stage of share c of `cuts`.
+__host__ __device__ inline int first_stage(int c, int cuts, int stages) {
+  return static_cast<int>(static_cast<long long>(c) * stages / cuts);
 }
 
-template <int NT, int MATS>
+template <int NT>
 __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_constant__ ThinParams p) {
-  using Cfg = ThinCfg<NT, MATS>;
+  using Cfg = ThinCfg<NT>;
   extern __shared__ uint8_t thin_smem[];
   __shared__ __align__(8) uint64_t bar_tma[8], bar_split[8], bar_empty[8], bar_tmem_full[2], bar_tmem_empty[2];
   __shared__ uint32_t tmem_slot;
@@ -100,11 +102,14 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // this run: `count` blocks from k-block k_first of column block item_first on (every role carries (item, k) along: a
-  // division per block would cost the issuing thread more than the products it issues)
-  const long long u0 = first_block(blockIdx.x, gridDim.x, p.blocks);
-  const int count = static_cast<int>(first_block(blockIdx.x + 1, gridDim.x, p.blocks) - u0);
-  const int item_first = static_cast<int>(u0 / p.kblocks), k_first = static_cast<int>(u0 - static_cast<long long>(item_first) * p.kblocks);
+  const int cuts = p.slices / p.items;
+  // every role walks this block's slices: body(item, first stage, stage behind the last, slice)
+  auto each_slice = [&](auto body) {
+    for (int id = blockIdx.x; id < p.slices; id += gridDim.x) {
+      const int c = id / p.items;
+      if (!body(id - c * p.items, first_stage(c, cuts, p.stages), first_stage(c + 1, cuts, p.stages), id)) break;
+    }
+  };
   auto give_up = [&](int role, int a, int b) {
     abort_flag = 1;
     atomicCAS(p.status, 0, (role << 24) | ((a & 0xFF) << 16) | (b & 0xFFFF));
@@ -115,41 +120,48 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
     if (warp == 0) {
       // ---------------------------------------------------------- loads
       uint32_t s = 0, ph = 0, it = 0;
-      uint32_t held = 0;                   // k-blocks whose X has not been asked for yet
+      uint32_t held = 0;                   // stages whose X has not been asked for yet
+      int held_k[R];
       bool started = p.early == 0;
       auto load_x = [&](uint32_t slot, int k) {
-        tma_load_3d(raw + slot * Cfg::RAW + Cfg::W_BYTES, &p.tmX, smem_u32(&bar_tma[slot]), k * 32, 0, 0, 0ull);
+#pragma unroll
+        for (int b = 0; b < Cfg::KS; ++b)
+          tma_load_3d(raw + slot * Cfg::RAW + Cfg::W_BYTES + b * 2 * Cfg::X_BYTES, &p.tmX, smem_u32(&bar_tma[slot]),
+                      (k * Cfg::KS + b) * 32, 0, 0, 0ull);
       };
       auto x_of_held = [&]() {             // weights may be asked for before X exists; X waits for the grid that writes it
         if (lane == 0) {
           asm volatile("griddepcontrol.wait;" ::: "memory");
-          for (uint32_t i = 0; i < held; ++i) load_x(i, (k_first + static_cast<int>(i)) % p.kblocks);
+          for (uint32_t i = 0; i < held; ++i) load_x(i, held_k[i]);
         }
         __syncwarp();
         started = true;
       };
-      int item = item_first, k = k_first;
-      for (; it < static_cast<uint32_t>(count); ++it) {
-        if (!started && held == R) x_of_held();
-        if (!mbar_wait(smem_u32(&bar_empty[s]), ph ^ 1u, &abort_flag)) {
-          if (lane == 0) give_up(ROLE_THIN_LOAD, s, it);
-          break;
-        }
-        if (elect_one()) {
-          const uint32_t bar = smem_u32(&bar_tma[s]), dst = raw + s * Cfg::RAW;
-          mbar_arrive_expect_tx(bar, Cfg::W_BYTES + Cfg::X_BYTES);
+      each_slice([&](int item, int k0, int k1, int) {
+        for (int k = k0; k < k1; ++k, ++it) {
+          if (!started && held == R) x_of_held();
+          if (!mbar_wait(smem_u32(&bar_empty[s]), ph ^ 1u, &abort_flag)) {
+            if (lane == 0) give_up(ROLE_THIN_LOAD, s, it);
+            return false;
+          }
+          if (elect_one()) {
+            const uint32_t bar = smem_u32(&bar_tma[s]), dst = raw + s * Cfg::RAW;
+            mbar_arrive_expect_tx(bar, Cfg::W_BYTES + Cfg::KS * Cfg::X_BYTES);
+            const CUtensorMap* map = item < p.blocks ? &p.tmW[0] : &p.tmW[1];
+            const int col = (item < p.blocks ? item : item - p.blocks) * 128;
 #pragma unroll
-          for (int m = 0; m < MATS; ++m)
+            for (int b = 0; b < Cfg::KS; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              tma_load_3d(dst + m * 16384 + j * 4096, &p.tmW[m], bar, item * 128 + j * 32, k * 32, 0, 0ull);
-          if (started) load_x(s, k);
+              for (int j = 0; j < 4; ++j)
+                tma_load_3d(dst + b * 16384 + j * 4096, map, bar, col + j * 32, (k * Cfg::KS + b) * 32, 0, 0ull);
+            if (started) load_x(s, k);
+          }
+          __syncwarp();
+          if (!started) held_k[held++] = k;
+          if (++s == R) { s = 0; ph ^= 1u; }
         }
-        __syncwarp();
-        if (!started) ++held;
-        if (++k == p.kblocks) { k = 0; ++item; }
-        if (++s == R) { s = 0; ph ^= 1u; }
-      }
+        return true;
+      });
       if (!started) x_of_held();
       if (lane == 0 && abort_flag) {       // copies in flight land before shared memory is released
         for (uint32_t i = it > R ? it - R : 0u; i < it; ++i) {
@@ -164,33 +176,31 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
       constexpr uint32_t ID_NT = make_idesc_tf32(128, NT, true, false);
       constexpr uint64_t A_STEP = 1024 >> 4, B_STEP = 32 >> 4;     // 8 rows of K
       uint32_t s = 0, ph = 0, l = 0, ch = 0;
-      int kk = 0, k = k_first;
-      for (int i = 0; i < count; ++i) {
-        if (++k == p.kblocks) k = 0;
-        const bool seg_end = k == 0 || i + 1 == count;
+      each_slice([&](int, int k0, int k1, int) {
+      for (int k = k0, kk = 0; k < k1; ++k) {
         const bool first = kk == 0;
-        const bool last = ++kk == p.kc || seg_end;
+        const bool last = ++kk == p.chunk || k + 1 == k1;
         if (last) kk = 0;
         if (!mbar_wait(smem_u32(&bar_split[s]), ph, &abort_flag)) {
-          if (lane == 0) give_up(ROLE_THIN_MMA, s, i);
-          break;
+          if (lane == 0) give_up(ROLE_THIN_MMA, s, k);
+          return false;
         }
         const uint32_t buf = ch & 1u;
         if (first && !mbar_wait(smem_u32(&bar_tmem_empty[buf]), ((ch >> 1) & 1u) ^ 1u, &abort_flag)) {
-          if (lane == 0) give_up(ROLE_THIN_MMA, 50 + buf, i);
-          break;
+          if (lane == 0) give_up(ROLE_THIN_MMA, 50 + buf, k);
+          return false;
         }
         tc_fence_after();
-        const uint32_t x = raw + s * Cfg::RAW + Cfg::W_BYTES;
         if (elect_one()) {
-          const uint64_t bx = make_smem_desc(x, 16u, 1024u, SMEM_LAYOUT_SW128);
-          const uint64_t bxl = make_smem_desc(x + Cfg::X_BYTES, 16u, 1024u, SMEM_LAYOUT_SW128);
-          const uint32_t fresh = first ? 0u : 1u;
+          const uint32_t d = tmem + buf * Cfg::DCOLS;
 #pragma unroll
-          for (int m = 0; m < MATS; ++m) {
-            const uint64_t a_hi = make_smem_desc(raw + s * Cfg::RAW + m * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
-            const uint64_t a_lo = make_smem_desc(lo + l * Cfg::LO + m * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
-            const uint32_t d = tmem + (buf * MATS + m) * Cfg::DCOLS;
+          for (int b = 0; b < Cfg::KS; ++b) {
+            const uint32_t x = raw + s * Cfg::RAW + Cfg::W_BYTES + b * 2 * Cfg::X_BYTES;
+            const uint64_t bx = make_smem_desc(x, 16u, 1024u, SMEM_LAYOUT_SW128);
+            const uint64_t bxl = make_smem_desc(x + Cfg::X_BYTES, 16u, 1024u, SMEM_LAYOUT_SW128);
+            const uint64_t a_hi = make_smem_desc(raw + s * Cfg::RAW + b * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
+            const uint64_t a_lo = make_smem_desc(lo + l * Cfg::LO + b * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
+            const uint32_t fresh = first && b == 0 ? 0u : 1u;
             if (Cfg::CONCAT) {
               // columns [0, NT): hi*hi; columns [NT, 2 NT): hi*lo, then lo*hi
 #pragma unroll
@@ -216,22 +226,33 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
         if (++l == L) l = 0;
         if (last) ++ch;
       }
+      return true;
+      });
     } else {
       // ---------------------------------------------------------- split
-      const int st = (warp - 2) * 32 + lane;
+      const uint32_t group = (warp - 2) / Cfg::SPLIT_WARPS;
+      const int st = ((warp - 2) % Cfg::SPLIT_WARPS) * 32 + lane;
       constexpr int NST = Cfg::SPLIT_WARPS * 32;
       constexpr int VW = Cfg::W_BYTES / 16, VX = Cfg::X_BYTES / 16;
       static_assert(VW % 32 == 0 && VX % 32 == 0, "a warp's 32 vectors are 512 contiguous bytes");
       uint32_t s = 0, ph = 0, l = 0, sp = 0, php = 0, it = 0;
-      for (; it < static_cast<uint32_t>(count); ++it) {
+      auto next_block = [&]() {
+        if (++s == R) { s = 0; ph ^= 1u; }
+        if (++l == L) l = 0;
+        if (it + 1 > L && ++sp == R) { sp = 0; php ^= 1u; }      // (sp, php): stage it + 1 - L
+        ++it;
+      };
+      each_slice([&](int, int k0, int k1, int) {
+      for (int k = k0; k < k1; ++k, next_block()) {
+        if (it % Cfg::GROUPS != group) continue;
         if (!mbar_wait(smem_u32(&bar_tma[s]), ph, &abort_flag)) {
           if (lane == 0) give_up(ROLE_THIN_SPLIT, s, it);
-          break;
+          return false;
         }
-        if (L != R && it >= L) {           // the lo slot is free once the products of k-block it - L are done
+        if (L != R && it >= L) {           // the lo slot is free once the products of stage it - L are done
           if (!mbar_wait(smem_u32(&bar_empty[sp]), php, &abort_flag)) {
             if (lane == 0) give_up(ROLE_THIN_SPLIT, 100 + sp, it);
-            break;
+            return false;
           }
         }
         const uint32_t from = raw + s * Cfg::RAW, to_w = lo + l * Cfg::LO;
@@ -255,71 +276,55 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
           }
         }
 #pragma unroll
-        for (int b = 0; b < (VX + NST - 1) / NST; ++b) {
-          const int v = st + b * NST;
-          if (v < VX) {
-            const float4 x = lds2x64(from + Cfg::W_BYTES + (v - lane) * 16, lane);
-            sts2x64(from + Cfg::W_BYTES + Cfg::X_BYTES + (v - lane) * 16, lane, lo_of(x));
+        for (int b = 0; b < (Cfg::KS * VX + NST - 1) / NST; ++b) {
+          const int v = st + b * NST, sub = v / VX;     // X of the sub-blocks, each with its lo part behind it
+          if (v < Cfg::KS * VX) {
+            const uint32_t at = from + Cfg::W_BYTES + sub * 2 * Cfg::X_BYTES + (v - sub * VX - lane) * 16;
+            sts2x64(at + Cfg::X_BYTES, lane, lo_of(lds2x64(at, lane)));
           }
         }
         fence_proxy_async_smem();          // the tensor core reads these through the async proxy
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_split[s]));
-        if (++s == R) { s = 0; ph ^= 1u; }
-        if (++l == L) l = 0;
-        if (it + 1 > L && ++sp == R) { sp = 0; php ^= 1u; }      // (sp, php): k-block it + 1 - L
       }
+      return true;
+      });
     }
   } else {
     // ------------------------------------------------------------ drain: tensor memory -> registers -> scratch
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_DRAINERS));
-    constexpr int MINE = Cfg::MINE;
-    const int q = warp & 3, m0 = MINE == MATS ? 0 : (warp - Cfg::DRAIN_WARP0) >> 2;
+    const int q = warp & 3;
     uint32_t ch = 0;
-    bool alive = true;
-    int item = item_first, k = k_first;
-    for (int i = 0; alive && i < count; ++item, k = 0) {
-      const int end = min(i + p.kblocks - k, count);
-      float acc[MINE][NT];
+    each_slice([&](int, int k0, int k1, int id) {
+      float acc[NT];
 #pragma unroll
-      for (int m = 0; m < MINE; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[m][t] = 0.0f;
-      for (; i < end; i += p.kc, ++ch) {
+      for (int t = 0; t < NT; ++t) acc[t] = 0.0f;
+      for (int k = k0; k < k1; k += p.chunk, ++ch) {
         const uint32_t buf = ch & 1u;
         if (!mbar_wait(smem_u32(&bar_tmem_full[buf]), (ch >> 1) & 1u, &abort_flag)) {
-          if (lane == 0) give_up(ROLE_THIN_DRAIN, buf, i);
-          alive = false;
-          break;
+          if (lane == 0) give_up(ROLE_THIN_DRAIN, buf, k);
+          return false;
         }
         tc_fence_after();
+        const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * Cfg::DCOLS;
 #pragma unroll
-        for (int m = 0; m < MINE; ++m) {
-          const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + (buf * MATS + m0 + m) * Cfg::DCOLS;
+        for (int t = 0; t < NT; t += 16) {
+          float big[16], small[16];
+          tmem_ld_32x16(at + t, big);
+          if (Cfg::CONCAT) tmem_ld_32x16(at + NT + t, small);
+          tmem_wait_ld();
 #pragma unroll
-          for (int t = 0; t < NT; t += 16) {
-            float big[16], small[16];
-            tmem_ld_32x16(at + t, big);
-            if (Cfg::CONCAT) tmem_ld_32x16(at + NT + t, small);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[m][t + j] += Cfg::CONCAT ? big[j] + small[j] : big[j];
-          }
+          for (int j = 0; j < 16; ++j) acc[t + j] += Cfg::CONCAT ? big[j] + small[j] : big[j];
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[buf]));
       }
-      i = end;
-      if (alive) {
-        // slot: run + item, which grows from one segment of the list to the next
-        float* out = p.part + ((static_cast<long long>(blockIdx.x) + item) * MATS + m0) * (NT * 128) + q * 32 + lane;
+      float* out = p.part + static_cast<long long>(id) * (NT * 128) + q * 32 + lane;
 #pragma unroll
-        for (int m = 0; m < MINE; ++m)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) out[(m * NT + t) * 128] = acc[m][t];
-      }
-    }
+      for (int t = 0; t < NT; ++t) out[t * 128] = acc[t];
+      return true;
+    });
   }
   tc_fence_before();
   __syncthreads();
@@ -329,12 +334,11 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
   }
 }
 
-// Sums of a column block's runs in order, gate, rows out.  One 16-byte vector of a row per thread.
+// Sums of a column block's slices in order, gate, rows out.  One 16-byte vector of a row per thread.
 struct ThinSumParams {
   const float* part;
   float* out; float* G; float* U;
-  int N, M, act, kblocks, runs;
-  long long blocks;
+  int N, M, act, blocks, cuts;
 };
 template <int NT, int MATS>
 __global__ void __launch_bounds__(256) thin_sum_kernel(const __grid_constant__ ThinSumParams p) {
@@ -344,17 +348,15 @@ __global__ void __launch_bounds__(256) thin_sum_kernel(const __grid_constant__ T
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < static_cast<long long>(p.N) * vecs;
        i += static_cast<long long>(gridDim.x) * 256) {
     const int n = static_cast<int>(i / vecs), v = static_cast<int>(i - static_cast<long long>(n) * vecs);
-    const int item = v >> 5;
-    const long long first = static_cast<long long>(item) * p.kblocks;
-    const int b0 = run_of(first, p.runs, p.blocks), b1 = run_of(first + p.kblocks - 1, p.runs, p.blocks);
+    const int block = v >> 5;
     float s[MATS * 4];
 #pragma unroll
     for (int k = 0; k < MATS * 4; ++k) s[k] = 0.0f;
-    for (int b = b0; b <= b1; ++b) {
+    for (int b = 0; b < p.cuts; ++b) {
 #pragma unroll
       for (int m = 0; m < MATS; ++m) {
         const float4 x = *reinterpret_cast<const float4*>(
-            p.part + (((static_cast<long long>(b) + item) * MATS + m) * NT + n) * 128 + (v & 31) * 4);
+            p.part + (((static_cast<long long>(b) * MATS + m) * p.blocks + block) * NT + n) * 128 + (v & 31) * 4);
         s[m * 4] += x.x; s[m * 4 + 1] += x.y; s[m * 4 + 2] += x.z; s[m * 4 + 3] += x.w;
       }
     }
@@ -370,16 +372,24 @@ __global__ void __launch_bounds__(256) thin_sum_kernel(const __grid_constant__ T
   }
 }
 
-int runs_of(long long blocks) {
-  // a run shorter than four k-blocks costs more in its sums than it saves
-  const long long most = device_sm_count(), want = (blocks + 3) / 4;
-  return static_cast<int>(want < most ? want : most);
+// Shares of K: the rounds of slices over the SMs times a slice's blocks of 32 rows (0.37 us of a block's way from memory
+// each, five more for a slice's start and end), plus what the slices' sums cost to write and read again.
+int cuts_of(int items, int kblocks, int rows) {
+  const int sms = device_sm_count();
+  int best = 1;
+  double best_t = 1e300;
+  for (int c = 1; c <= 32 && (c == 1 || kblocks / c >= 4); ++c) {
+    const int rounds = (items * c + sms - 1) / sms;
+    const double t = rounds * ((kblocks + c - 1) / c + 5) * 0.37e-6 + static_cast<double>(items) * c * rows * 128 * 8 / 4e12;
+    if (t < best_t) { best_t = t; best = c; }
+  }
+  return best;
 }
 
 template <int NT, int MATS>
 int thin_launch(const ThinCall& c, cudaStream_t st) {
-  using Cfg = ThinCfg<NT, MATS>;
-  auto kernel = thin_kernel<NT, MATS>;
+  using Cfg = ThinCfg<NT>;
+  auto kernel = thin_kernel<NT>;
   static std::atomic<int> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -397,19 +407,22 @@ int thin_launch(const ThinCall& c, cudaStream_t st) {
     if (int rc = make_map3(&p.tmW[1], c.W1, m, k, 1, m, m * k, 32, 32, true)) return rc;
   if (int rc = make_map3(&p.tmX, c.X, k, n, 1, k, k * n, 32, NT, false)) return rc;
   p.part = c.work;
-  p.kblocks = (c.K + 31) / 32;
-  p.items = (c.M + 127) / 128;
-  p.blocks = static_cast<long long>(p.kblocks) * p.items;
-  p.kc = tuned_kc();
+  const int kblocks = (c.K + 31) / 32;
+  p.stages = (kblocks + Cfg::KS - 1) / Cfg::KS;
+  p.blocks = (c.M + 127) / 128;
+  p.items = p.blocks * MATS;
+  const int cuts = cuts_of(p.items, kblocks, NT);
+  p.slices = p.items * cuts;
+  p.chunk = tuned_kc() / Cfg::KS > 1 ? tuned_kc() / Cfg::KS : 1;
   p.early = c.early;
   p.status = status_word_ptr(&e);
   if (!p.status) return static_cast<int>(e);
-  const int runs = runs_of(p.blocks);
+  const int grid_x = p.slices < device_sm_count() ? p.slices : device_sm_count();
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(runs, 1, 1);
+  cfg.gridDim = dim3(grid_x, 1, 1);
   cfg.blockDim = dim3(THIN_THREADS, 1, 1);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = st;
@@ -419,7 +432,7 @@ int thin_launch(const ThinCall& c, cudaStream_t st) {
   if (e != cudaSuccess) return static_cast<int>(e);
   ThinSumParams q{};
   q.part = c.work; q.out = c.out; q.G = c.G; q.U = c.U;
-  q.N = c.N; q.M = c.M; q.act = c.act; q.kblocks = p.kblocks; q.runs = runs; q.blocks = p.blocks;
+  q.N = c.N; q.M = c.M; q.act = c.act; q.blocks = p.blocks; q.cuts = cuts;
   const long long vecs = static_cast<long long>(c.N) * (c.M / 4);
   long long grid = (vecs + 255) / 256;
   if (grid > 8LL * device_sm_count()) grid = 8LL * device_sm_count();
@@ -435,8 +448,8 @@ int thin_rows(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; 
 }  // namespace
 
 long long thin_work_floats(int N, int M, int K, int mats) {
-  const long long items = (M + 127) / 128, blocks = items * ((K + 31) / 32);
-  return (runs_of(blocks) + items - 1) * mats * thin_rows(N) * 128;
+  const int items = (M + 127) / 128 * mats;
+  return static_cast<long long>(items) * cuts_of(items, (K + 31) / 32, thin_rows(N)) * thin_rows(N) * 128;
 }
 
 int thin_product(const ThinCall& c, cudaStream_t st) {
