@@ -34,35 +34,42 @@ struct ThinParams {
   float* part;              // [slice][row][128 columns]
   int stages, items, slices, chunk;    // slice id: share of K * items + item; items: column blocks, matrix by matrix;
                                        // K in stages of 32 KS rows, `chunk` of them summed in tensor memory
-  int blocks;                          // column blocks of a matrix
+  int blocks;                          // column blocks of a matrix (items of both matrices at once: as many items)
   int early;                // the grid may start before the one that writes X has ended
   int* status;
 };
 
-template <int NT>
+// MP: matrices per slice.  Up to 32 rows a slice is of one matrix and a stage of the ring holds two blocks of it; beyond, X
+// and its split weigh as much as the weights, and a gated slice takes the same block of both matrices against one X.
+template <int NT, int MP>
 struct ThinCfg {
   static constexpr bool CONCAT = NT <= 64;
   // Rows of 32 per stage of the ring.  What a stage costs whatever its size - the issuing thread's waits and commits, the
   // split's fence - is 700 cycles, the time 16 KB take from memory: two rows of blocks share it where the ring allows.
   static constexpr int KS = NT <= 32 ? 2 : 1;
-  static constexpr int W_BYTES = KS * 16384;                      // weights of a stage
+  static constexpr int SUBS = KS * MP;                            // 16 KB weight tiles of a stage
+  static constexpr int W_BYTES = SUBS * 16384;
   static constexpr int X_BYTES = NT * 128;                        // X of 32 rows of K; its lo part behind it
   static constexpr int RAW = W_BYTES + KS * 2 * X_BYTES;
   static constexpr int LO = W_BYTES;                              // lo part of the weights
   // A lo slot is held from the split until the products that read it are seen to be done.
-  static constexpr int L = KS == 2 ? 2 : 3;
+  static constexpr int L = SUBS == 2 ? 2 : 3;
   static constexpr int FIT = (225 * 1024 - L * LO) / RAW;
   static constexpr int R = FIT < 8 ? FIT : 8;
   static constexpr int SMEM = 1024 + R * RAW + L * LO;
   static constexpr int DCOLS = CONCAT ? 2 * NT : NT;              // tensor-memory columns per buffer
-  static constexpr int TMEM_COLS = 2 * DCOLS <= 64 ? 64 : 2 * DCOLS <= 128 ? 128 : 256;
-  // Four drain warps hold all sums of their 32 columns.  Ten of the sixteen warps split: all on one stage, or, where a
-  // stage is small, in groups of five that take the stages in turn (a split is mostly latency).
-  static constexpr int DRAIN_WARPS = 4, DRAIN_WARP0 = 16 - DRAIN_WARPS, GROUPS = KS == 2 ? 1 : 2,
-                       SPLIT_WARPS = (DRAIN_WARP0 - 2) / GROUPS;
-  static constexpr int REGS_MOVERS = 96, REGS_DRAINERS = 216;     // per thread after reallocation, 64 K in all
+  static constexpr int TMEM_NEED = 2 * MP * DCOLS;
+  static constexpr int TMEM_COLS = TMEM_NEED <= 64 ? 64 : TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
+  // Four drain warps hold all sums of their 32 columns where those are 128 at most, else eight, a matrix each half.  The
+  // other warps but two split: all on one stage, or, where a stage is one tile, in two groups that take the stages in turn
+  // (a split is mostly latency).
+  static constexpr int DRAIN_WARPS = MP * NT <= 128 ? 4 : 8, DRAIN_WARP0 = 16 - DRAIN_WARPS;
+  static constexpr int MINE = DRAIN_WARPS == 4 ? MP : 1;          // matrices per drain warp
+  static constexpr int GROUPS = SUBS == 2 ? 1 : 2, SPLIT_WARPS = (DRAIN_WARP0 - 2) / GROUPS;
+  // registers per thread after reallocation, 64 K in all
+  static constexpr int REGS_MOVERS = DRAIN_WARPS == 4 ? 96 : 72, REGS_DRAINERS = DRAIN_WARPS == 4 ? 216 : 184;
   static_assert(REGS_MOVERS * DRAIN_WARP0 * 32 + REGS_DRAINERS * DRAIN_WARPS * 32 <= 65536, "registers");
-  static_assert(R >= L && 2 * DCOLS <= 256 && SMEM <= 227 * 1024 - 512, "thin");
+  static_assert(R >= L && TMEM_NEED <= 512 && SMEM <= 227 * 1024 - 512, "thin");
 };
 
 // First stage of share c of `cuts`.
@@ -70,9 +77,9 @@ __host__ __device__ inline int first_stage(int c, int cuts, int stages) {
   return static_cast<int>(static_cast<long long>(c) * stages / cuts);
 }
 
-template <int NT>
+template <int NT, int MP>
 __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_constant__ ThinParams p) {
-  using Cfg = ThinCfg<NT>;
+  using Cfg = ThinCfg<NT, MP>;
   extern __shared__ uint8_t thin_smem[];
   __shared__ __align__(8) uint64_t bar_tma[8], bar_split[8], bar_empty[8], bar_tmem_full[2], bar_tmem_empty[2];
   __shared__ uint32_t tmem_slot;
@@ -147,13 +154,15 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
           if (elect_one()) {
             const uint32_t bar = smem_u32(&bar_tma[s]), dst = raw + s * Cfg::RAW;
             mbar_arrive_expect_tx(bar, Cfg::W_BYTES + Cfg::KS * Cfg::X_BYTES);
-            const CUtensorMap* map = item < p.blocks ? &p.tmW[0] : &p.tmW[1];
-            const int col = (item < p.blocks ? item : item - p.blocks) * 128;
+            const bool other = MP == 1 && item >= p.blocks;
+            const int col = (other ? item - p.blocks : item) * 128;
 #pragma unroll
-            for (int b = 0; b < Cfg::KS; ++b)
+            for (int b = 0; b < Cfg::SUBS; ++b) {
+              const CUtensorMap* map = (MP == 2 ? b == 1 : other) ? &p.tmW[1] : &p.tmW[0];
+              const int row = (MP == 2 ? k : k * Cfg::KS + b) * 32;
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                tma_load_3d(dst + b * 16384 + j * 4096, map, bar, col + j * 32, (k * Cfg::KS + b) * 32, 0, 0ull);
+              for (int j = 0; j < 4; ++j) tma_load_3d(dst + b * 16384 + j * 4096, map, bar, col + j * 32, row, 0, 0ull);
+            }
             if (started) load_x(s, k);
           }
           __syncwarp();
@@ -192,15 +201,15 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
         }
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t d = tmem + buf * Cfg::DCOLS;
 #pragma unroll
-          for (int b = 0; b < Cfg::KS; ++b) {
-            const uint32_t x = raw + s * Cfg::RAW + Cfg::W_BYTES + b * 2 * Cfg::X_BYTES;
+          for (int b = 0; b < Cfg::SUBS; ++b) {
+            const uint32_t d = tmem + (buf * MP + (MP == 2 ? b : 0)) * Cfg::DCOLS;
+            const uint32_t x = raw + s * Cfg::RAW + Cfg::W_BYTES + (MP == 2 ? 0 : b) * 2 * Cfg::X_BYTES;
             const uint64_t bx = make_smem_desc(x, 16u, 1024u, SMEM_LAYOUT_SW128);
             const uint64_t bxl = make_smem_desc(x + Cfg::X_BYTES, 16u, 1024u, SMEM_LAYOUT_SW128);
             const uint64_t a_hi = make_smem_desc(raw + s * Cfg::RAW + b * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
             const uint64_t a_lo = make_smem_desc(lo + l * Cfg::LO + b * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
-            const uint32_t fresh = first && b == 0 ? 0u : 1u;
+            const uint32_t fresh = first && (MP == 2 || b == 0) ? 0u : 1u;
             if (Cfg::CONCAT) {
               // columns [0, NT): hi*hi; columns [NT, 2 NT): hi*lo, then lo*hi
 #pragma unroll
@@ -293,12 +302,15 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
   } else {
     // ------------------------------------------------------------ drain: tensor memory -> registers -> scratch
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_DRAINERS));
-    const int q = warp & 3;
+    constexpr int MINE = Cfg::MINE;
+    const int q = warp & 3, m0 = MINE == MP ? 0 : (warp - Cfg::DRAIN_WARP0) >> 2;
     uint32_t ch = 0;
     each_slice([&](int, int k0, int k1, int id) {
-      float acc[NT];
+      float acc[MINE][NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] = 0.0f;
+      for (int m = 0; m < MINE; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[m][t] = 0.0f;
       for (int k = k0; k < k1; k += p.chunk, ++ch) {
         const uint32_t buf = ch & 1u;
         if (!mbar_wait(smem_u32(&bar_tmem_full[buf]), (ch >> 1) & 1u, &abort_flag)) {
@@ -306,23 +318,28 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
           return false;
         }
         tc_fence_after();
-        const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * Cfg::DCOLS;
 #pragma unroll
-        for (int t = 0; t < NT; t += 16) {
-          float big[16], small[16];
-          tmem_ld_32x16(at + t, big);
-          if (Cfg::CONCAT) tmem_ld_32x16(at + NT + t, small);
-          tmem_wait_ld();
+        for (int m = 0; m < MINE; ++m) {
+          const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + (buf * MP + m0 + m) * Cfg::DCOLS;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) acc[t + j] += Cfg::CONCAT ? big[j] + small[j] : big[j];
+          for (int t = 0; t < NT; t += 16) {
+            float big[16], small[16];
+            tmem_ld_32x16(at + t, big);
+            if (Cfg::CONCAT) tmem_ld_32x16(at + NT + t, small);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[m][t + j] += Cfg::CONCAT ? big[j] + small[j] : big[j];
+          }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[buf]));
       }
-      float* out = p.part + static_cast<long long>(id) * (NT * 128) + q * 32 + lane;
+      float* out = p.part + (static_cast<long long>(id) * MP + m0) * (NT * 128) + q * 32 + lane;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) out[t * 128] = acc[t];
+      for (int m = 0; m < MINE; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) out[(m * NT + t) * 128] = acc[m][t];
       return true;
     });
   }
@@ -334,13 +351,16 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
   }
 }
 
+// Matrices a gated slice takes.
+constexpr int mats_per_slice(int rows) { return rows >= 64 ? 2 : 1; }
+
 // Sums of a column block's slices in order, gate, rows out.  One 16-byte vector of a row per thread.
 struct ThinSumParams {
   const float* part;
   float* out; float* G; float* U;
   int N, M, act, blocks, cuts;
 };
-template <int NT, int MATS>
+template <int NT, int MATS, bool TOGETHER>      // TOGETHER: the slices held both matrices
 __global__ void __launch_bounds__(256) thin_sum_kernel(const __grid_constant__ ThinSumParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -352,11 +372,15 @@ __global__ void __launch_bounds__(256) thin_sum_kernel(const __grid_constant__ T
     float s[MATS * 4];
 #pragma unroll
     for (int k = 0; k < MATS * 4; ++k) s[k] = 0.0f;
+    auto part_of = [&](int c, int m, int blk) -> long long {
+      return TOGETHER ? (static_cast<long long>(c) * p.blocks + blk) * 2 + m
+                      : (static_cast<long long>(c) * MATS + m) * p.blocks + blk;
+    };
     for (int b = 0; b < p.cuts; ++b) {
 #pragma unroll
       for (int m = 0; m < MATS; ++m) {
         const float4 x = *reinterpret_cast<const float4*>(
-            p.part + (((static_cast<long long>(b) * MATS + m) * p.blocks + block) * NT + n) * 128 + (v & 31) * 4);
+            p.part + (part_of(b, m, block) * NT + n) * 128 + (v & 31) * 4);
         s[m * 4] += x.x; s[m * 4 + 1] += x.y; s[m * 4 + 2] += x.z; s[m * 4 + 3] += x.w;
       }
     }
@@ -374,13 +398,14 @@ __global__ void __launch_bounds__(256) thin_sum_kernel(const __grid_constant__ T
 
 // Shares of K: the rounds of slices over the SMs times a slice's blocks of 32 rows (0.37 us of a block's way from memory
 // each, five more for a slice's start and end), plus what the slices' sums cost to write and read again.
-int cuts_of(int items, int kblocks, int rows) {
+int cuts_of(int items, int kblocks, int rows, int mats) {
   const int sms = device_sm_count();
   int best = 1;
   double best_t = 1e300;
   for (int c = 1; c <= 32 && (c == 1 || kblocks / c >= 4); ++c) {
     const int rounds = (items * c + sms - 1) / sms;
-    const double t = rounds * ((kblocks + c - 1) / c + 5) * 0.37e-6 + static_cast<double>(items) * c * rows * 128 * 8 / 4e12;
+    const double t = rounds * ((kblocks + c - 1) / c + 5) * mats * 0.37e-6 +
+                     static_cast<double>(items) * c * mats * rows * 128 * 8 / 4e12;
     if (t < best_t) { best_t = t; best = c; }
   }
   return best;
@@ -388,8 +413,9 @@ int cuts_of(int items, int kblocks, int rows) {
 
 template <int NT, int MATS>
 int thin_launch(const ThinCall& c, cudaStream_t st) {
-  using Cfg = ThinCfg<NT>;
-  auto kernel = thin_kernel<NT>;
+  constexpr int MP = MATS == 2 ? mats_per_slice(NT) : 1;
+  using Cfg = ThinCfg<NT, MP>;
+  auto kernel = thin_kernel<NT, MP>;
   static std::atomic<int> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -410,8 +436,8 @@ int thin_launch(const ThinCall& c, cudaStream_t st) {
   const int kblocks = (c.K + 31) / 32;
   p.stages = (kblocks + Cfg::KS - 1) / Cfg::KS;
   p.blocks = (c.M + 127) / 128;
-  p.items = p.blocks * MATS;
-  const int cuts = cuts_of(p.items, kblocks, NT);
+  p.items = p.blocks * MATS / MP;
+  const int cuts = cuts_of(p.items, kblocks, NT, MP);
   p.slices = p.items * cuts;
   p.chunk = tuned_kc() / Cfg::KS > 1 ? tuned_kc() / Cfg::KS : 1;
   p.early = c.early;
@@ -440,7 +466,7 @@ int thin_launch(const ThinCall& c, cudaStream_t st) {
   cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, thin_sum_kernel<NT, MATS>, q));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, thin_sum_kernel<NT, MATS, MP == 2>, q));
 }
 
 int thin_rows(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; }
@@ -448,8 +474,9 @@ int thin_rows(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; 
 }  // namespace
 
 long long thin_work_floats(int N, int M, int K, int mats) {
-  const int items = (M + 127) / 128 * mats;
-  return static_cast<long long>(items) * cuts_of(items, (K + 31) / 32, thin_rows(N)) * thin_rows(N) * 128;
+  const int rows = thin_rows(N), together = mats == 2 ? mats_per_slice(rows) : 1;
+  const int items = (M + 127) / 128 * mats / together;
+  return static_cast<long long>(items) * cuts_of(items, (K + 31) / 32, rows, together) * together * rows * 128;
 }
 
 int thin_product(const ThinCall& c, cudaStream_t st) {
