@@ -7,7 +7,9 @@ Modules
 -------
 build    nvcc recipe for ``libdragon_cu32.so``
 cu32     ctypes binding that mirrors the Java native classes ``Cuda_matMul``,
-         ``Cuda_batchMatMul`` and ``Cuda_conv3D`` (same method names and argument order)
+         ``Cuda_batchMatMul`` and ``Cuda_conv3D`` (same method names and argument order),
+         and the classes of the transformer operators (``Cuda_gatedFF``,
+         ``Cuda_normResidual``, ``Cuda_gradClip``)
 engine   host-side mirror of the parts of ``CudaFloat32EngineBase`` that call those
          natives (split-K decision, stream count, padded dimensions)
 shard    one-process-per-GPU sharding of the three operator families

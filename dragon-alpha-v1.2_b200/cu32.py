@@ -182,9 +182,11 @@ def _p(addr):
     return ctypes.cast(ctypes.c_void_p(int(addr)), _fp)
 
 
+_S10 = c_int64 * 10
+
+
 def _streams(streamArray, length):
-    arr = (c_int64 * 10)(*([int(s) for s in streamArray[:10]] + [0] * (10 - min(len(streamArray), 10))))
-    return arr, int(length)
+    return _S10(*[int(s) for s in streamArray[:10]]), int(length)      # the rest are zero
 
 
 def _check(rc, where):
@@ -213,7 +215,8 @@ def decode_status(word: int) -> str:
     if word == 0:
         return "ok"
     roles = {1: "tma-producer", 2: "splitter", 3: "mma(operands)", 4: "mma(tmem-buffer)", 5: "drainer",
-             7: "self-test"}
+             7: "self-test", 8: "norm(row)", 9: "norm(sum)", 10: "rows(load)", 11: "rows(tile)", 12: "rows(sum)",
+             13: "thin(load)", 14: "thin(split)", 15: "thin(mma)", 16: "thin(drain)"}
     return f"{roles.get(word >> 24, word >> 24)} gave up at stage/buffer {(word >> 16) & 0xFF}, iteration {word & 0xFFFF}"
 
 
@@ -843,13 +846,13 @@ class Cuda_gradClip:
     @staticmethod
     def gradNorm(stream, src, sizes, count, dResult, dWork, work_doubles):
         """dResult[0] = norm, dResult[1] = 1."""
-        a, z = Cuda_gradClip._ints(src, count), Cuda_gradClip._ints(sizes, count)
+        a, z = Cuda_gradClip._ints(src, count), Cuda_gradClip._ints(sizes, count)   # alive until the call returns
         _check(load().cu32_gradNorm(stream, a.buffer_info()[0], z.buffer_info()[0], count, dResult, dWork, work_doubles),
                "gradNorm")
 
     @staticmethod
     def gradClip(stream, src, dst, sizes, count, max_norm, dResult, dWork, work_doubles):
         """dst = src * min(1, max_norm / norm); dResult = {norm, factor}."""
-        a, b, z = (Cuda_gradClip._ints(v, count) for v in (src, dst, sizes))
+        a, b, z = Cuda_gradClip._ints(src, count), Cuda_gradClip._ints(dst, count), Cuda_gradClip._ints(sizes, count)
         _check(load().cu32_gradClip(stream, a.buffer_info()[0], b.buffer_info()[0], z.buffer_info()[0], count, max_norm,
                                     dResult, dWork, work_doubles), "gradClip")

@@ -15,7 +15,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
-from .cu32 import Cuda_batchMatMul, Cuda_conv3D, Cuda_matMul
+from .cu32 import Cuda_batchMatMul, Cuda_conv3D, Cuda_gatedFF, Cuda_gradClip, Cuda_matMul, Cuda_normResidual
 
 
 def pad4(x: int) -> int:
@@ -281,6 +281,51 @@ class Cu32Engine:
         if GridZ > 1:
             dw.buf_summary(self.streams[0], buf, deltaW, GridZ - 1, size)
         return GridZ
+
+    # ---- operators of transformer layers (no counterpart in the Java engine); scratch comes from the pool like the split
+    # products' partial buffers, optional addresses are 0
+    def _scratch(self, nfloats):
+        if nfloats <= 0:
+            return 0
+        addr, keep = self.malloc(nfloats)
+        self._keep.append(keep)
+        return addr
+
+    def gatedFF(self, Y, X, Wg, Wu, Wd, N, D, F, act, H=0, G=0, U=0):
+        """Y = (act(X Wg) * (X Wu)) Wd.  Training keeps H, G = X Wg and U = X Wu; serving leaves them out."""
+        work = Cuda_gatedFF.work(N, D, F)
+        Cuda_gatedFF.gatedFF(self.streams[:1], 1, X, Wg, Wu, Wd, G, U, H or self._scratch(N * F), Y, self._scratch(work), work,
+                             N, D, F, act)
+
+    def gatedFF_delta(self, deltaX, deltaWg, deltaWu, deltaWd, deltaY, X, Wg, Wu, Wd, G, U, H, N, D, F, act):
+        """Gradients of gatedFF from what its forward call kept; any of the four may be 0 (not computed).  U is replaced
+        by deltaU (no later product needs it)."""
+        work = Cuda_gatedFF.work(N, D, F)
+        Cuda_gatedFF.gatedFF_delta(self.streams[:1], 1, deltaY, X, Wg, Wu, Wd, G, U, H, self._scratch(N * F), U, deltaX, deltaWg,
+                                   deltaWu, deltaWd, self._scratch(work), work, N, D, F, act)
+
+    def normResidual(self, Rout, Y, B, R, Wpre, N, M, width, Wpost=0, gate=0, gate_rows=0, res_scale=1.0, scale=1.0, eps=1e-6,
+                     rstd_post=0, rstd_pre=0):
+        """R' = res_scale R + scale gate (Wpost B / rms(B)), Y = Wpre R' / rms(R')."""
+        Cuda_normResidual.normResidual(self.streams[0], B, R, gate, gate_rows, Wpost, Wpre, Rout, Y, rstd_post, rstd_pre, N, M,
+                                       width, res_scale, scale, eps)
+
+    def normResidual_delta(self, deltaR, deltaB, deltaWpre, deltaRout, deltaY, B, Rout, Wpre, rstd_pre, N, M, width, Wpost=0,
+                           rstd_post=0, deltaWpost=0, gate=0, gate_rows=0, deltaGate=0, res_scale=1.0, scale=1.0):
+        work = Cuda_normResidual.work(N, M, gate_rows if gate else 0)
+        Cuda_normResidual.normResidual_delta(self.streams[0], deltaRout, deltaY, B, Rout, gate, gate_rows, Wpost, Wpre, rstd_post,
+                                             rstd_pre, deltaR, deltaB, deltaGate, deltaWpost, deltaWpre, self._scratch(work),
+                                             work, N, M, width, res_scale, scale)
+
+    def gradNorm(self, src, sizes, result):
+        """result[0] = sqrt of the sum of squares over all tensors."""
+        work = Cuda_gradClip.work(len(sizes))
+        Cuda_gradClip.gradNorm(self.streams[0], src, sizes, len(sizes), result, self._scratch(2 * work), work)
+
+    def gradClip(self, src, dst, sizes, max_norm, result):
+        """dst = src * min(1, max_norm / norm) over all tensors; result = {norm, factor}."""
+        work = Cuda_gradClip.work(len(sizes))
+        Cuda_gradClip.gradClip(self.streams[0], src, dst, sizes, len(sizes), max_norm, result, self._scratch(2 * work), work)
 
     def release(self):
         """Drop the workspaces (the Java Syncer frees them after the streams complete)."""
