@@ -165,7 +165,6 @@ static int pick_tile(long long M, int N, long long z) {
 // Ring lengths for a launch (see GemmParams): explicit tuning values win, otherwise 0 = the kernel
 // configuration's balanced default.
 // Also sets how many chunks are summed in registers between flushes to memory: 256 k-blocks (K = 8192).
-int tuned_kc() { return g_kc.load(); }
 int forced_tile() { return g_tile.load(); }
 void choose_rings(GemmParams* p) {
   p->flush_chunks = 256 / p->kc > 1 ? 256 / p->kc : 1;
@@ -236,7 +235,7 @@ int run_gemm(const GemmCall& c) {
   p.tiles_m = (c.M + 128 * ctas - 1) / (128 * ctas);
   p.tiles_n = (c.n_store + bn - 1) / bn;
   p.gz = c.gz;
-  p.kc = c.x3 ? g_kc.load() : g_kc_fast.load();
+  p.kc = c.kc > 0 ? c.kc : c.x3 ? g_kc.load() : g_kc_fast.load();
   choose_rings(&p);
   if (below_ridge && p.ring_raw == 0) {
     if (tile == TILE_1x64) { p.ring_raw = 6; p.ring_lo = 2; p.store_bufs = 1; }

@@ -31,6 +31,7 @@ struct GemmCall {
   float alpha = 1.0f;
   float* const* replicas = nullptr;   // further output buffers that receive the same stores as C (same layout)
   int n_replicas = 0;
+  int kc = 0;                         // k-blocks per in-TMEM chunk; 0 = the "kc" tuning keys
   bool beside_prev = false;           // may run beside the previous launch on the stream, which it does not depend on
 };
 
@@ -47,8 +48,10 @@ int make_map3(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint6
               uint64_t pitch2_floats, uint32_t b0, uint32_t b1, bool mn_major);
 int make_map3_as(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t pitch1_floats,
                  uint64_t pitch2_floats, uint32_t b0, uint32_t b1, CUtensorMapSwizzle swizzle);
-// k-blocks per in-TMEM chunk of the FP32-accurate mode (the "kc" tuning key).
-int tuned_kc();
+// k-blocks per in-TMEM chunk of the gated block's products.  Their errors add up along the block (G, U, H, Y and back), and
+// the tensor core's truncation grows with the chunk: with one the block's results are 6e-7 off, with two (the plain
+// products' default) 1.3e-6, for 2 to 5 % of its time.
+constexpr int GATED_KC = 1;
 // The "tile" tuning key: a forced tile configuration, or -1.
 int forced_tile();
 // Ring lengths, flush interval, clock accumulator and reserved SMs of a launch, from the tuning integers.

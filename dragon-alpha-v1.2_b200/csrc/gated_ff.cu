@@ -529,7 +529,7 @@ int product(const int64_t* s, bool a_mn, bool b_mn, const float* A, long long ld
   const int nkb = (K + 31) / 32;
   const ColumnPlan plan = plan_columns(PLAIN_TILES, 6, M, N, nkb, 1);
   c.gz = split_of(PLAIN_TILES, 6, M, N, nkb, work ? room : 0, plan.time);
-  c.x3 = true; c.stream = st;
+  c.x3 = true; c.stream = st; c.kc = GATED_KC;
   c.beside_prev = beside && c.gz == 1;
   if (c.gz > 1) {
     if (int rc = run_gemm(c)) return rc;
@@ -552,7 +552,7 @@ int fill_common(GemmParams* p, int M, int N, int nkb, int tile, int out_bn) {
   p->tiles_m = (M + 128 * tile_ctas(tile) - 1) / (128 * tile_ctas(tile));
   p->tiles_n = (N + out_bn - 1) / out_bn;
   p->gz = 1;
-  p->kc = tuned_kc();
+  p->kc = GATED_KC;
   choose_rings(p);
   p->vec4_ok = 1;
   cudaError_t e;

@@ -6,7 +6,7 @@
 // are therefore exchanged against the general contraction kernel: 128 weight columns are the rows of the tensor core's
 // tile (operand A, MN-major as they lie), the NT rows of X its columns - no tile row is wasted on rows X does not have.
 // Arithmetic as there: hi = what the tensor core makes of an FP32 operand, lo = rounded remainder, written beside it by
-// split warps; lo*hi + hi*lo + hi*hi, at most `kc` k-blocks summed in tensor memory before FP32 registers take over.
+// split warps; lo*hi + hi*lo + hi*hi, a stage of the ring summed in tensor memory before FP32 registers take over.
 // Up to 64 rows X's lo part lies right behind its hi part, so that one instruction with 2 NT columns forms hi*hi and hi*lo
 // and the weight tile is fetched twice per step instead of three times (the fetches from shared memory bound the step).
 //
@@ -439,7 +439,7 @@ int thin_launch(const ThinCall& c, cudaStream_t st) {
   p.items = p.blocks * MATS / MP;
   const int cuts = cuts_of(p.items, kblocks, NT, MP);
   p.slices = p.items * cuts;
-  p.chunk = tuned_kc() / Cfg::KS > 1 ? tuned_kc() / Cfg::KS : 1;
+  p.chunk = (GATED_KC + Cfg::KS - 1) / Cfg::KS;
   p.early = c.early;
   p.status = status_word_ptr(&e);
   if (!p.status) return static_cast<int>(e);
