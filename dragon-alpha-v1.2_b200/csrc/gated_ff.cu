@@ -656,8 +656,12 @@ int check_dims(int N, int D, int F, int act) {
 }
 
 long long thin_floats(int N, int D, int F) {
-  const long long up = thin_work_floats(N, F, D, 2), down = thin_work_floats(N, D, F, 1);
+  const long long up = thin_work_floats(N, F, D, THIN_GATED), down = thin_work_floats(N, D, F, THIN_PLAIN);
   return up > down ? up : down;
+}
+long long thin_delta_floats(int N, int D, int F) {
+  const long long h = thin_work_floats(N, F, D, THIN_DELTA), x = thin_work_floats(N, D, F, THIN_DUAL);
+  return h > x ? h : x;
 }
 
 template <class... P>
@@ -682,10 +686,11 @@ long long cu32_gatedFF_work(int N, int D, int F) {
   const long long c = extra(split_of(PLAIN_TILES, 6, d, f, (N + 31) / 32, any), d * f);       // deltaWg, deltaWu
   const long long e = extra(split_of(PLAIN_TILES, 6, f, d, (N + 31) / 32, any), d * f);       // deltaWd
   const long long m = a > b ? a : b, o = c > e ? c : e;
-  const long long most = m > o ? m : o;
-  if (N <= ROWS_MAX || N > THIN_MAX_ROWS) return most;
-  const long long thin = thin_floats(N, D, F);
-  return thin > most ? thin : most;
+  long long most = m > o ? m : o;
+  if (N > THIN_MAX_ROWS) return most;
+  const long long forward = N > ROWS_MAX ? thin_floats(N, D, F) : 0, backward = thin_delta_floats(N, D, F);
+  if (forward > most) most = forward;
+  return backward > most ? backward : most;
 }
 
 int cu32_gatedFF(const int64_t* s, int length, const float* X, const float* Wg, const float* Wu, const float* Wd, float* G,
@@ -703,10 +708,10 @@ int cu32_gatedFF(const int64_t* s, int length, const float* X, const float* Wg, 
     return rows_any<1>(down, st);
   }
   if (N <= THIN_MAX_ROWS && work && thin_floats(N, D, F) <= work_floats) {
-    const ThinCall up{X, Wg, Wu, H, G, U, work, N, F, D, act, 0};
-    if (int rc = thin_product(up, st)) return rc;
-    const ThinCall down{H, Wd, nullptr, Y, nullptr, nullptr, work, N, D, F, 0, 1};
-    return thin_product(down, st);
+    const ThinCall up{X, nullptr, Wg, Wu, H, G, U, nullptr, nullptr, work, N, F, D, act, 0};
+    if (int rc = thin_product(up, THIN_GATED, st)) return rc;
+    const ThinCall down{H, nullptr, Wd, nullptr, Y, nullptr, nullptr, nullptr, nullptr, work, N, D, F, 0, 1};
+    return thin_product(down, THIN_PLAIN, st);
   }
   if (int rc = gated_tiles(X, Wg, Wu, G, U, H, N, D, F, act, st)) return rc;
   return product(s, false, true, H, F, Wd, D, Y, N, D, F, work, work_floats, st);
@@ -727,14 +732,23 @@ int cu32_gatedFF_delta(const int64_t* s, int length, const float* dY, const floa
   // the one before: deltaWd with deltaH, and deltaWg with deltaWu.
   if (dWd)
     if (int rc = product(s, true, true, H, F, dY, D, dWd, F, D, N, work, work_floats, st)) return rc;
-  if (int rc = product(s, false, false, dY, D, Wd, D, dG, N, F, D, work, work_floats, st, dWd != nullptr && dG != H)) return rc;
-  const long long vecs = static_cast<long long>(N) * F / 4;
-  long long blocks = (vecs + 511) / 512;
-  if (blocks > 16LL * device_sm_count()) blocks = 16LL * device_sm_count();
-  gated_delta_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(dG, dU, G, U, vecs, act);
-  if (cudaError_t e = cudaPeekAtLastError()) return static_cast<int>(e);
-  if (dX)
-    if (int rc = dual_tiles(s, dG, Wg, dU, Wu, dX, N, D, F, work, work_floats, st)) return rc;
+  if (N <= THIN_MAX_ROWS && work && thin_delta_floats(N, D, F) <= work_floats) {
+    const ThinCall h{dY, nullptr, Wd, nullptr, dG, nullptr, dU, G, U, work, N, F, D, act, 0};
+    if (int rc = thin_product(h, THIN_DELTA, st)) return rc;
+    if (dX) {
+      const ThinCall x{dG, dU, Wg, Wu, dX, nullptr, nullptr, nullptr, nullptr, work, N, D, F, 0, 1};
+      if (int rc = thin_product(x, THIN_DUAL, st)) return rc;
+    }
+  } else {
+    if (int rc = product(s, false, false, dY, D, Wd, D, dG, N, F, D, work, work_floats, st, dWd != nullptr && dG != H)) return rc;
+    const long long vecs = static_cast<long long>(N) * F / 4;
+    long long blocks = (vecs + 511) / 512;
+    if (blocks > 16LL * device_sm_count()) blocks = 16LL * device_sm_count();
+    gated_delta_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(dG, dU, G, U, vecs, act);
+    if (cudaError_t e = cudaPeekAtLastError()) return static_cast<int>(e);
+    if (dX)
+      if (int rc = dual_tiles(s, dG, Wg, dU, Wu, dX, N, D, F, work, work_floats, st)) return rc;
+  }
   if (dWg)
     if (int rc = product(s, true, true, X, D, dG, F, dWg, D, F, N, work, work_floats, st, false)) return rc;
   if (dWu)

@@ -1,4 +1,4 @@
-// Products of 9 to 128 rows with a large weight (gemm_thin.cu).
+// Products of up to 128 rows with a large weight (gemm_thin.cu).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -6,15 +6,21 @@ namespace dragon {
 
 constexpr int THIN_MAX_ROWS = 128;
 
-// out[N, M] = X[N, K] W0[K, M], or act(X W0) * (X W1) with the pre-activations in G and U when G is not null.
+enum ThinForm {
+  THIN_PLAIN,      // out[N, M] = X[N, K] W0[K, M]
+  THIN_GATED,      // out = act(X W0) * (X W1), the pre-activations in G and U when G is not null
+  THIN_DELTA,      // h[N, M] = X[N, K] W0[M, K]^T; out = h * preU * act'(preG), U = h * act(preG)
+  THIN_DUAL,       // out[N, M] = X W0[M, K]^T + X1 W1[M, K]^T
+};
 struct ThinCall {
-  const float* X; const float* W0; const float* W1;
+  const float* X; const float* X1; const float* W0; const float* W1;
   float* out; float* G; float* U;
+  const float* preG; const float* preU;
   float* work;              // thin_work_floats of scratch
   int N, M, K, act;
   int early;                // X is written by the launch before, a dependent of which this one may be
 };
-long long thin_work_floats(int N, int M, int K, int mats);
-int thin_product(const ThinCall& c, cudaStream_t st);
+long long thin_work_floats(int N, int M, int K, ThinForm form);
+int thin_product(const ThinCall& c, ThinForm form, cudaStream_t st);
 
 }  // namespace dragon

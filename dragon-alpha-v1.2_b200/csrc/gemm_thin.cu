@@ -1,10 +1,11 @@
 // Products of a few dozen rows with a large weight, FP32-accurate on the tensor cores:
-//   out[n, :] = X[n, :] W   or   act(X[n, :] W0) * (X[n, :] W1),   9 to 128 rows.
+//   out[n, :] = X[n, :] W   or   act(X[n, :] W0) * (X[n, :] W1),   9 to 128 rows, and for the gradients
+//   deltaG, deltaU from deltaH = deltaY W^T,   deltaX = deltaG W0^T + deltaU W1^T,   up to 128 rows.
 //
 // Every weight is read once for all rows, so the time should be that of reading the weights (with the general kernel it was
 // three times that: 315 us for 16 rows of a 4096 / 10924 block, 537 MB).  The roles of the operands
 // are therefore exchanged against the general contraction kernel: 128 weight columns are the rows of the tensor core's
-// tile (operand A, MN-major as they lie), the NT rows of X its columns - no tile row is wasted on rows X does not have.
+// tile (operand A as they lie: MN-major, or K-major for W^T), the NT rows of X its columns - no tile row is wasted on rows X does not have.
 // Arithmetic as there: hi = what the tensor core makes of an FP32 operand, lo = rounded remainder, written beside it by
 // split warps; lo*hi + hi*lo + hi*hi, a stage of the ring summed in tensor memory before FP32 registers take over.
 // Up to 64 rows X's lo part lies right behind its hi part, so that one instruction with 2 NT columns forms hi*hi and hi*lo
@@ -29,8 +30,9 @@ constexpr int THIN_THREADS = 512;
 constexpr int ROLE_THIN_LOAD = 13, ROLE_THIN_SPLIT = 14, ROLE_THIN_MMA = 15, ROLE_THIN_DRAIN = 16;
 
 struct ThinParams {
-  CUtensorMap tmW[2];       // [K, M] weights, boxes of 32 x 32 (MN-major slabs)
-  CUtensorMap tmX;          // [N, K], boxes of NT rows x 32 (K-major)
+  CUtensorMap tmW[2];       // [K, M] weights, boxes of 32 x 32 (MN-major slabs), or [M, K], boxes of 128 rows x 32
+  CUtensorMap tmX[2];       // [N, K], boxes of NT rows x 32 (K-major); the second only for two products in one sum
+  int half;                 // two products in one sum: stages of the first, else the number of stages
   float* part;              // [slice][row][128 columns]
   int stages, items, slices, chunk;    // slice id: share of K * items + item; items: column blocks, matrix by matrix;
                                        // K in stages of 32 KS rows, `chunk` of them summed in tensor memory
@@ -41,7 +43,7 @@ struct ThinParams {
 
 // MP: matrices per slice.  Up to 32 rows a slice is of one matrix and a stage of the ring holds two blocks of it; beyond, X
 // and its split weigh as much as the weights, and a gated slice takes the same block of both matrices against one X.
-template <int NT, int MP>
+template <int NT, int MP, bool A_KM = false>
 struct ThinCfg {
   static constexpr bool CONCAT = NT <= 64;
   // Rows of 32 per stage of the ring.  What a stage costs whatever its size - the issuing thread's waits and commits, the
@@ -77,9 +79,9 @@ __host__ __device__ inline int first_stage(int c, int cuts, int stages) {
   return static_cast<int>(static_cast<long long>(c) * stages / cuts);
 }
 
-template <int NT, int MP>
+template <int NT, int MP, bool A_KM>      // A_KM: the weights are [M, K]
 __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_constant__ ThinParams p) {
-  using Cfg = ThinCfg<NT, MP>;
+  using Cfg = ThinCfg<NT, MP, A_KM>;
   extern __shared__ uint8_t thin_smem[];
   __shared__ __align__(8) uint64_t bar_tma[8], bar_split[8], bar_empty[8], bar_tmem_full[2], bar_tmem_empty[2];
   __shared__ uint32_t tmem_slot;
@@ -131,10 +133,12 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
       int held_k[R];
       bool started = p.early == 0;
       auto load_x = [&](uint32_t slot, int k) {
+        const CUtensorMap* map = k >= p.half ? &p.tmX[1] : &p.tmX[0];
+        const int k0 = (k >= p.half ? k - p.half : k) * Cfg::KS * 32;
 #pragma unroll
         for (int b = 0; b < Cfg::KS; ++b)
-          tma_load_3d(raw + slot * Cfg::RAW + Cfg::W_BYTES + b * 2 * Cfg::X_BYTES, &p.tmX, smem_u32(&bar_tma[slot]),
-                      (k * Cfg::KS + b) * 32, 0, 0, 0ull);
+          tma_load_3d(raw + slot * Cfg::RAW + Cfg::W_BYTES + b * 2 * Cfg::X_BYTES, map, smem_u32(&bar_tma[slot]), k0 + b * 32, 0, 0,
+                      0ull);
       };
       auto x_of_held = [&]() {             // weights may be asked for before X exists; X waits for the grid that writes it
         if (lane == 0) {
@@ -154,14 +158,18 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
           if (elect_one()) {
             const uint32_t bar = smem_u32(&bar_tma[s]), dst = raw + s * Cfg::RAW;
             mbar_arrive_expect_tx(bar, Cfg::W_BYTES + Cfg::KS * Cfg::X_BYTES);
-            const bool other = MP == 1 && item >= p.blocks;
-            const int col = (other ? item - p.blocks : item) * 128;
+            const bool other = MP == 1 && item >= p.blocks, later = k >= p.half;
+            const int col = (other ? item - p.blocks : item) * 128, kk = later ? k - p.half : k;
 #pragma unroll
             for (int b = 0; b < Cfg::SUBS; ++b) {
-              const CUtensorMap* map = (MP == 2 ? b == 1 : other) ? &p.tmW[1] : &p.tmW[0];
-              const int row = (MP == 2 ? k : k * Cfg::KS + b) * 32;
+              const CUtensorMap* map = (MP == 2 ? b == 1 : other || later) ? &p.tmW[1] : &p.tmW[0];
+              const int row = (MP == 2 ? kk : kk * Cfg::KS + b) * 32;
+              if (A_KM) {
+                tma_load_3d(dst + b * 16384, map, bar, row, col, 0, 0ull);
+              } else {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) tma_load_3d(dst + b * 16384 + j * 4096, map, bar, col + j * 32, row, 0, 0ull);
+                for (int j = 0; j < 4; ++j) tma_load_3d(dst + b * 16384 + j * 4096, map, bar, col + j * 32, row, 0, 0ull);
+              }
             }
             if (started) load_x(s, k);
           }
@@ -181,9 +189,11 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------- products
-      constexpr uint32_t ID_WIDE = make_idesc_tf32(128, Cfg::CONCAT ? 2 * NT : NT, true, false);
-      constexpr uint32_t ID_NT = make_idesc_tf32(128, NT, true, false);
-      constexpr uint64_t A_STEP = 1024 >> 4, B_STEP = 32 >> 4;     // 8 rows of K
+      constexpr uint32_t ID_WIDE = make_idesc_tf32(128, Cfg::CONCAT ? 2 * NT : NT, !A_KM, false);
+      constexpr uint32_t ID_NT = make_idesc_tf32(128, NT, !A_KM, false);
+      constexpr uint32_t A_LBO = A_KM ? 16u : 4096u, A_SBO = A_KM ? 1024u : 512u;
+      constexpr uint32_t A_LT = A_KM ? SMEM_LAYOUT_SW128 : SMEM_LAYOUT_SW128_32B;
+      constexpr uint64_t A_STEP = (A_KM ? 32 : 1024) >> 4, B_STEP = 32 >> 4;     // 8 rows of K
       uint32_t s = 0, ph = 0, l = 0, ch = 0;
       each_slice([&](int, int k0, int k1, int) {
       for (int k = k0, kk = 0; k < k1; ++k) {
@@ -207,8 +217,8 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) thin_kernel(const __grid_cons
             const uint32_t x = raw + s * Cfg::RAW + Cfg::W_BYTES + (MP == 2 ? 0 : b) * 2 * Cfg::X_BYTES;
             const uint64_t bx = make_smem_desc(x, 16u, 1024u, SMEM_LAYOUT_SW128);
             const uint64_t bxl = make_smem_desc(x + Cfg::X_BYTES, 16u, 1024u, SMEM_LAYOUT_SW128);
-            const uint64_t a_hi = make_smem_desc(raw + s * Cfg::RAW + b * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
-            const uint64_t a_lo = make_smem_desc(lo + l * Cfg::LO + b * 16384, 4096u, 512u, SMEM_LAYOUT_SW128_32B);
+            const uint64_t a_hi = make_smem_desc(raw + s * Cfg::RAW + b * 16384, A_LBO, A_SBO, A_LT);
+            const uint64_t a_lo = make_smem_desc(lo + l * Cfg::LO + b * 16384, A_LBO, A_SBO, A_LT);
             const uint32_t fresh = first && (MP == 2 || b == 0) ? 0u : 1u;
             if (Cfg::CONCAT) {
               // columns [0, NT): hi*hi; columns [NT, 2 NT): hi*lo, then lo*hi
@@ -358,6 +368,7 @@ constexpr int mats_per_slice(int rows) { return rows >= 64 ? 2 : 1; }
 struct ThinSumParams {
   const float* part;
   float* out; float* G; float* U;
+  const float* preG; const float* preU;      // gradients: the pre-activations; out, U = deltaG, deltaU
   int N, M, act, blocks, cuts;
 };
 template <int NT, int MATS, bool TOGETHER>      // TOGETHER: the slices held both matrices
@@ -392,6 +403,16 @@ __global__ void __launch_bounds__(256) thin_sum_kernel(const __grid_constant__ T
       }
       gated_forward<4>(p.act, s);
     }
+    if constexpr (MATS == 1) {
+      if (p.preG != nullptr) {               // s is deltaH
+        const float4 g = *reinterpret_cast<const float4*>(p.preG + at), u = *reinterpret_cast<const float4*>(p.preU + at);
+        float4 dg, du;
+        gated_backward4(p.act, make_float4(s[0], s[1], s[2], s[3]), g, u, &dg, &du);
+        *reinterpret_cast<float4*>(p.out + at) = dg;
+        *reinterpret_cast<float4*>(p.U + at) = du;
+        continue;
+      }
+    }
     *reinterpret_cast<float4*>(p.out + at) = make_float4(s[0], s[1], s[2], s[3]);
   }
 }
@@ -411,11 +432,12 @@ int cuts_of(int items, int kblocks, int rows, int mats) {
   return best;
 }
 
-template <int NT, int MATS>
+// MATS matrices side by side, or (A_KM) the transposed ones, two of them summed.
+template <int NT, int MATS, bool A_KM>
 int thin_launch(const ThinCall& c, cudaStream_t st) {
   constexpr int MP = MATS == 2 ? mats_per_slice(NT) : 1;
-  using Cfg = ThinCfg<NT, MP>;
-  auto kernel = thin_kernel<NT, MP>;
+  using Cfg = ThinCfg<NT, MP, A_KM>;
+  auto kernel = thin_kernel<NT, MP, A_KM>;
   static std::atomic<int> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -428,16 +450,22 @@ int thin_launch(const ThinCall& c, cudaStream_t st) {
   ThinParams p;
   std::memset(&p, 0, sizeof(p));
   const uint64_t n = c.N, k = c.K, m = c.M;
-  if (int rc = make_map3(&p.tmW[0], c.W0, m, k, 1, m, m * k, 32, 32, true)) return rc;
-  if (MATS == 2)
-    if (int rc = make_map3(&p.tmW[1], c.W1, m, k, 1, m, m * k, 32, 32, true)) return rc;
-  if (int rc = make_map3(&p.tmX, c.X, k, n, 1, k, k * n, 32, NT, false)) return rc;
+  auto weight_map = [&](CUtensorMap* map, const float* w) {
+    return A_KM ? make_map3(map, w, k, m, 1, k, k * m, 32, 128, false) : make_map3(map, w, m, k, 1, m, m * k, 32, 32, true);
+  };
+  if (int rc = weight_map(&p.tmW[0], c.W0)) return rc;
+  if (c.W1)
+    if (int rc = weight_map(&p.tmW[1], c.W1)) return rc;
+  if (int rc = make_map3(&p.tmX[0], c.X, k, n, 1, k, k * n, 32, NT, false)) return rc;
+  if (c.X1)
+    if (int rc = make_map3(&p.tmX[1], c.X1, k, n, 1, k, k * n, 32, NT, false)) return rc;
   p.part = c.work;
   const int kblocks = (c.K + 31) / 32;
-  p.stages = (kblocks + Cfg::KS - 1) / Cfg::KS;
+  p.half = (kblocks + Cfg::KS - 1) / Cfg::KS;
+  p.stages = c.X1 ? 2 * p.half : p.half;
   p.blocks = (c.M + 127) / 128;
   p.items = p.blocks * MATS / MP;
-  const int cuts = cuts_of(p.items, kblocks, NT, MP);
+  const int cuts = cuts_of(p.items, c.X1 ? 2 * kblocks : kblocks, NT, MP);
   p.slices = p.items * cuts;
   p.chunk = (GATED_KC + Cfg::KS - 1) / Cfg::KS;
   p.early = c.early;
@@ -457,7 +485,7 @@ int thin_launch(const ThinCall& c, cudaStream_t st) {
   e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) return static_cast<int>(e);
   ThinSumParams q{};
-  q.part = c.work; q.out = c.out; q.G = c.G; q.U = c.U;
+  q.part = c.work; q.out = c.out; q.G = c.G; q.U = c.U; q.preG = c.preG; q.preU = c.preU;
   q.N = c.N; q.M = c.M; q.act = c.act; q.blocks = p.blocks; q.cuts = cuts;
   const long long vecs = static_cast<long long>(c.N) * (c.M / 4);
   long long grid = (vecs + 255) / 256;
@@ -473,20 +501,25 @@ int thin_rows(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; 
 
 }  // namespace
 
-long long thin_work_floats(int N, int M, int K, int mats) {
-  const int rows = thin_rows(N), together = mats == 2 ? mats_per_slice(rows) : 1;
-  const int items = (M + 127) / 128 * mats / together;
-  return static_cast<long long>(items) * cuts_of(items, (K + 31) / 32, rows, together) * together * rows * 128;
+long long thin_work_floats(int N, int M, int K, ThinForm form) {
+  const int rows = thin_rows(N), mats = form == THIN_GATED ? 2 : 1, together = form == THIN_GATED ? mats_per_slice(rows) : 1;
+  const int items = (M + 127) / 128 * mats / together, kblocks = (K + 31) / 32 * (form == THIN_DUAL ? 2 : 1);
+  return static_cast<long long>(items) * cuts_of(items, kblocks, rows, together) * together * rows * 128;
 }
 
-int thin_product(const ThinCall& c, cudaStream_t st) {
+int thin_product(const ThinCall& c, ThinForm form, cudaStream_t st) {
   if (!load_driver_entry_points()) return CU32_E_DRIVER;
-  const bool gated = c.W1 != nullptr;
-  switch (thin_rows(c.N)) {
-    case 16: return gated ? thin_launch<16, 2>(c, st) : thin_launch<16, 1>(c, st);
-    case 32: return gated ? thin_launch<32, 2>(c, st) : thin_launch<32, 1>(c, st);
-    case 64: return gated ? thin_launch<64, 2>(c, st) : thin_launch<64, 1>(c, st);
-    default: return gated ? thin_launch<128, 2>(c, st) : thin_launch<128, 1>(c, st);
+  const int rows = thin_rows(c.N);
+  switch (form) {
+    case THIN_GATED:
+      return rows == 16 ? thin_launch<16, 2, false>(c, st) : rows == 32 ? thin_launch<32, 2, false>(c, st)
+             : rows == 64 ? thin_launch<64, 2, false>(c, st) : thin_launch<128, 2, false>(c, st);
+    case THIN_PLAIN:
+      return rows == 16 ? thin_launch<16, 1, false>(c, st) : rows == 32 ? thin_launch<32, 1, false>(c, st)
+             : rows == 64 ? thin_launch<64, 1, false>(c, st) : thin_launch<128, 1, false>(c, st);
+    default:
+      return rows == 16 ? thin_launch<16, 1, true>(c, st) : rows == 32 ? thin_launch<32, 1, true>(c, st)
+             : rows == 64 ? thin_launch<64, 1, true>(c, st) : thin_launch<128, 1, true>(c, st);
   }
 }
 
