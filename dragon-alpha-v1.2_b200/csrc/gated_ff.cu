@@ -4,11 +4,16 @@
 //   deltaH = deltaY Wd^T;  deltaG = deltaH * U * act'(G);  deltaU = deltaH * act(G)
 //   deltaX = deltaG Wg^T + deltaU Wu^T;  deltaWg = X^T deltaG;  deltaWu = X^T deltaU;  deltaWd = H^T deltaY
 //
-// Many rows: the contraction kernel (gemm_tf32.cuh) with three epilogues of its own - both projections in one launch
-// with act(G) * U formed in the registers that hold the sums, deltaH turned into deltaG and deltaU before it is stored,
-// and the two products of deltaX in one accumulation.  6 N D F flop forward and 12 N D F backward at the
-// FP32-accurate rate bound it.
-// Few rows: every weight is read once for all rows, so the time is that of reading 3 D F floats; rows_kernel below.
+// Three forms, by what bounds them:
+// Up to 8 rows, forward: every weight is read once for all rows by FP32 multiply-adds, so the time is that of reading
+//   3 D F floats (rows_kernel below; 4096 / 10924, 537 MB: 93 us for one row, 103 us for 8).  The multiply-adds fill the
+//   issue slots beyond: 16 rows would take as long as two calls.
+// Up to 128 rows: the same reading bounds it, but the products run on the tensor cores with the weights as the tile's
+//   rows (gemm_thin.cu; 16 rows 117 us, 128 rows 251 us, where the tiles below take 315 and 320 us); it needs scratch.
+//   The gradients use it from one row on.
+// More rows: the contraction kernel (gemm_tf32.cuh) with both projections in one launch and act(G) * U formed in the
+//   registers that hold the sums, and with the two products of deltaX in one accumulation.  6 N D F flop forward and
+//   12 N D F backward at the FP32-accurate rate bound it.
 #include <atomic>
 
 #include "cu32_host.h"
@@ -94,8 +99,8 @@ struct RowsCfg {
 // columns, with the KT columns of X that meet them) full by TMA whatever the workers do; the persistent cluster takes
 // blocks of CPW columns in turn, its S blocks a slice of K each.  A worker holds 4 columns x NR rows of sums; the sums of
 // lanes, warps and blocks are added in a fixed order, each block of the cluster finishing CPW / S columns.
-// (Measured with plain loads into registers instead of the ring, one launch over all column blocks: 184 us for 8 rows of
-// a 4096 / 10924 layer, 537 MB.)
+// (Measured for 8 rows of a 4096 / 10924 block, 537 MB: 103 us, 5.2 TB/s; with plain loads into registers instead of the
+// ring, one launch over all column blocks, 184 us.)
 template <int NR, int MATS, int CPW, int S>
 __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_constant__ RowsParams p) {
   using Cfg = RowsCfg<NR, MATS, CPW, S>;

@@ -783,7 +783,7 @@ class Cuda_gatedFF:
 
     @staticmethod
     def work(N, D, F) -> int:
-        """Floats of scratch that let every product of the two calls be split as far as it would."""
+        """Floats of scratch the two calls can use (fewer, or none: slower)."""
         return load().cu32_gatedFF_work(N, D, F)
 
     @staticmethod
@@ -795,7 +795,7 @@ class Cuda_gatedFF:
     @staticmethod
     def gatedFF_delta(streamArray, length, d_deltaY, dX, dWg, dWu, dWd, dG, dU, dH, d_deltaG, d_deltaU, d_deltaX,
                       d_deltaWg, d_deltaWu, d_deltaWd, dWork, work_floats, N, D, F, act):
-        """deltaG and deltaU always (they may replace G and U), the others where they are given."""
+        """deltaG and deltaU always (deltaG may replace H, deltaU G or U), the others where they are given."""
         s, n = _streams(streamArray, length)
         _check(load().cu32_gatedFF_delta(s, n, d_deltaY, dX, dWg, dWu, dWd, dG, dU, dH, d_deltaG, d_deltaU, d_deltaX,
                                          d_deltaWg, d_deltaWu, d_deltaWd, dWork, work_floats, N, D, F, act),

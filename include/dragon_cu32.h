@@ -433,18 +433,23 @@ CU32_API int cu32_batchMatMulT2_softmax(const int64_t* streams, int length, cons
  *   every base pointer 16-byte aligned.  act: one of CU32_ACT_*, applied to G.
  * cu32_gatedFF
  *   G and U are written for the gradient call when given; both null in serving.  H is always written.
- *   Up to 8 rows the weights are read once for all rows (FP32 multiply-adds); more rows run on the tensor cores, both
- *   projections, the activation and the product in one kernel.
+ *   Up to 8 rows the weights are read once for all rows (FP32 multiply-adds, no scratch); up to 128 rows the same on the
+ *   tensor cores, through the scratch; more rows, or no scratch: both projections, the activation and the product in one
+ *   kernel.  The three round differently, so a row's bits depend on the form (not on the rows beside it).
  * cu32_gatedFF_delta
  *   deltaH = deltaY Wd^T, deltaG = deltaH * U * act'(G), deltaU = deltaH * act(G), both written; deltaU may be G or U and
- *   deltaG may be H, which are then replaced (deltaG must not be G, U or deltaU: CU32_E_ARG); deltaX = deltaG Wg^T + deltaU Wu^T, deltaWg = X^T deltaG, deltaWu = X^T deltaU,
- *   deltaWd = H^T deltaY.  deltaX, deltaWg, deltaWu and deltaWd may each be null: that gradient is not computed (and
- *   the operands only it needs may be null).
- * work: work_floats floats of scratch for split reductions, or null / 0 (products are then not split); its contents
- *   mean nothing between calls, and calls that may overlap need scratch of their own.  cu32_gatedFF_work says how many
- *   floats let every product of the two calls split as far as it would.
+ *   deltaG may be H, which are then replaced (deltaG must not be G, U or deltaU: CU32_E_ARG).  deltaX = deltaG Wg^T +
+ *   deltaU Wu^T, deltaWg = X^T deltaG, deltaWu = X^T deltaU, deltaWd = H^T deltaY.  deltaX, deltaWg, deltaWu and deltaWd
+ *   may each be null: that gradient is not computed (and the operands only it needs may be null).
+ * Apart from these replacements no output may overlap an operand or another output.
+ * work: work_floats floats of scratch for partial sums, or null / 0 (slower); its contents mean nothing between calls.
+ *   Calls that may overlap, and graphs that may be replayed side by side, need scratch of their own.  cu32_gatedFF_work
+ *   says how many floats the two calls can use; with fewer they give correct results more slowly.
+ * The products sum one k-block (32 terms) at a time inside the tensor core, whatever the "kc" tuning key says.
  * All outputs are fully overwritten; results do not vary from run to run (no atomics).  An infinite pre-activation
- * gives what the formula gives (NaN for SILU at -inf). */
+ * gives what the formula gives (NaN for SILU at -inf).  An infinity or NaN among the operands reaches the rows and columns
+ * whose sums it enters and no others; on the tensor cores such a sum is NaN, also where the formula's is infinite.
+ * Make the first call on each device outside any stream capture. */
 #define CU32_ACT_SILU 0        /* x / (1 + e^-x) */
 #define CU32_ACT_GELU 1        /* x Phi(x) */
 #define CU32_ACT_GELU_TANH 2   /* x / (1 + e^(-2 z)), z = sqrt(2/pi) (x + 0.044715 x^3) */
@@ -474,7 +479,8 @@ CU32_API long long cu32_gatedFF_work(int N, int D, int F);
  * cu32_normResidual_delta: from deltaRout (null = 0) and deltaY the gradients deltaR, deltaB, deltaGate (as gate),
  *   deltaWpost and deltaWpre [M]; the outputs of operands that were null are not touched and may be null.  deltaR may
  *   be deltaRout or deltaY, deltaB the other.  work: cu32_normResidual_work floats of scratch
- *   (fewer, down to 3 M, run with fewer thread blocks; below that CU32_E_SCRATCH).
+ *   (fewer, down to 3 M, run with fewer thread blocks; below that CU32_E_SCRATCH); calls that may overlap need their own.
+ * Apart from the replacements named no output may overlap an operand or another output.
  * Results do not vary from run to run (no atomics).  eps >= 0; with eps = 0 a row of zeros gives NaN. */
 CU32_API int cu32_normResidual(int64_t stream, const float* dB, const float* dR, const float* dGate, int gate_rows,
                                const float* dWpost, const float* dWpre, float* dRout, float* dY, float* dRstdPost,
@@ -491,7 +497,8 @@ CU32_API int cu32_normResidual_delta(int64_t stream, const float* d_deltaRout, c
  * norm = sqrt(sum of g^2 over all tensors), squares and sums in 64 bits; factor = max_norm / norm where norm > max_norm,
  * else 1; dst = src * factor.  No counterpart among the reference's natives.
  *   src, dst: host arrays of `count` device addresses (4-byte aligned; dst[i] may be src[i], anything else must not
- *   overlap), sizes: host array of their float counts (0 allowed).  The arrays are read during the call only.
+ *   overlap: in clipping a tensor is listed once), sizes: host array of their float counts (0 allowed).  The arrays are
+ *   read during the call only.
  *   result: two device floats, {norm, factor}.  A tensor that stays in place is not touched where the factor is 1.
  *   A norm that is not finite (an infinity or NaN among the gradients) gives factor 1: nothing is scaled, and the caller
  *   sees the norm.  max_norm >= 0 (infinity allowed).

@@ -387,3 +387,43 @@ def test_rows_do_not_depend_on_their_company(pkg, cuda):
         b.backward(pkg, 0)
         dX = b.get(torch, "dX")
         assert torch.isnan(dX[2]).all() and torch.isfinite(dX[others]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [4, 40, 128, 140])
+def test_bad_weights_stay_in_their_column(pkg, cuda, rows):
+    """A NaN weight reaches its hidden unit, whose H makes the rows of Y and, through deltaG, of deltaX NaN; no other column
+    of G, U, H, deltaG or of the weights' gradients."""
+    torch = cuda
+    b = Block(torch, rows, 68, 132, seed=19)
+    work = torch.empty(pkg.cu32.Cuda_gatedFF.work(rows, 68, 132) + 4, device="cuda")
+    b.Wg[7, 33] = float("nan")
+    b.forward(pkg, 0, work=work)
+    b.backward(pkg, 0, work=work)
+    others = [f for f in range(132) if f != 33]
+    for name in ("G", "H", "dG", "dU", "dWg", "dWu"):
+        t = b.get(torch, name)
+        assert torch.isnan(t[:, 33]).all() and torch.isfinite(t[:, others]).all(), name
+    assert torch.isfinite(b.get(torch, "U")).all()
+    dWd = b.get(torch, "dWd")
+    assert torch.isnan(dWd[33]).all() and torch.isfinite(dWd[others]).all()
+    for name in ("Y", "dX"):
+        assert torch.isnan(b.get(torch, name)).all(), name
+
+
+@pytest.mark.gpu
+def test_gradients_of_rows_do_not_depend_on_their_company_with_scratch(pkg, cuda):
+    """An infinity in one row of deltaY stays in that row of deltaG, deltaU and deltaX."""
+    torch = cuda
+    for rows in (1, 5, 40, 128, 140):
+        b = Block(torch, rows, 68, 132, seed=29)
+        work = torch.empty(pkg.cu32.Cuda_gatedFF.work(rows, 68, 132) + 4, device="cuda")
+        b.forward(pkg, 0, work=work)
+        b.backward(pkg, 0, work=work)
+        clean = {n: b.get(torch, n) for n in ("dG", "dU", "dX")}
+        b.dY[rows // 2, 5] = float("inf")
+        b.backward(pkg, 0, work=work)
+        others = [i for i in range(rows) if i != rows // 2]
+        for n, was in clean.items():
+            now = b.get(torch, n)
+            assert not torch.isfinite(now[rows // 2]).any() and torch.equal(now[others], was[others]), n
