@@ -272,7 +272,9 @@ int run_gemm(const GemmCall& c) {
   p.status = status_word_ptr(&e);
   if (!p.status) return static_cast<int>(e);
 
-  p.overlap_prev = p.join_prev = c.beside_prev ? 1 : 0;
+  p.overlap_prev = c.beside_prev || c.behind_prev ? 1 : 0;
+  p.join_prev = c.beside_prev ? 1 : 0;
+  p.wait_prev = c.behind_prev && !c.beside_prev ? 1 : 0;
   // Batches (or split-K slices) are folded into the kernel's tile index.
   const int zs = c.gz > 1 ? c.gz : c.batch;
   if (c.n_replicas > 0)       e = launch_gemm_rep(c.b_mn, p, zs, c.stream);

@@ -33,6 +33,7 @@ struct GemmCall {
   int n_replicas = 0;
   int kc = 0;                         // k-blocks per in-TMEM chunk; 0 = the "kc" tuning keys
   bool beside_prev = false;           // may run beside the previous launch on the stream, which it does not depend on
+  bool behind_prev = false;           // the previous launch on the stream is this call's own: start up beside its end
 };
 
 int run_gemm(const GemmCall& c);

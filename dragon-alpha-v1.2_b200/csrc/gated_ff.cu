@@ -521,11 +521,18 @@ ColumnPlan plan_columns(const int* tiles, int count, long long M, int N, int nkb
   return best;
 }
 
-// C[M,N] = op(A) op(B) through the plain contraction, cut along K or along its columns where that pays.
-// beside: it may share the machine with the previous launch (whose last tiles leave SMs idle) - only where that launch
-// neither writes what this one reads nor reads what it writes, and the product is not cut along K (the scratch is one).
+// Where a launch stands to the one before it on the stream.
+enum Order {
+  AFTER,       // behind it entirely: the first launch of a call
+  BEHIND,      // depends on it, a launch of the same call: only the start-up overlaps its end
+  BESIDE,      // may share the machine with it (whose last tiles leave SMs idle): it neither writes what this one reads nor
+               // reads what it writes, and has itself waited for whatever this one depends on
+};
+
+// C[M,N] = op(A) op(B) through the plain contraction, cut along K or along its columns where that pays.  A product cut along
+// K is never BESIDE the previous launch (the scratch is one).
 int product(const int64_t* s, bool a_mn, bool b_mn, const float* A, long long lda, const float* B, long long ldb, float* C,
-            int M, int N, int K, float* work, long long room, cudaStream_t st, bool beside = false) {
+            int M, int N, int K, float* work, long long room, cudaStream_t st, Order order) {
   GemmCall c{};
   c.A = A; c.B = B; c.C = C; c.Cbuf = work;
   c.M = M; c.N = N; c.K = K; c.n_store = N;
@@ -535,7 +542,8 @@ int product(const int64_t* s, bool a_mn, bool b_mn, const float* A, long long ld
   const ColumnPlan plan = plan_columns(PLAIN_TILES, 6, M, N, nkb, 1);
   c.gz = split_of(PLAIN_TILES, 6, M, N, nkb, work ? room : 0, plan.time);
   c.x3 = true; c.stream = st; c.kc = GATED_KC;
-  c.beside_prev = beside && c.gz == 1;
+  c.beside_prev = order == BESIDE && c.gz == 1;
+  c.behind_prev = order != AFTER;
   if (c.gz > 1) {
     if (int rc = run_gemm(c)) return rc;
     return sum_slices(s[0], C, work, c.gz, c.sC);
@@ -605,6 +613,8 @@ int gated_tiles(const float* X, const float* Wg, const float* Wu, float* G, floa
 // Each thread reads its elements before it writes them, so deltaU may lie over G or U.
 __global__ void __launch_bounds__(256) gated_delta_kernel(float* dG, float* dU, const float* G, const float* U, long long vecs,
                                                           int act) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
   for (long long v = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; v < vecs; v += 2 * stride) {
     const bool two = v + stride < vecs;
@@ -636,6 +646,7 @@ int dual_tiles(const int64_t* s, const float* dG, const float* Wg, const float* 
   std::memset(&p, 0, sizeof(p));
   const uint64_t n = N, d = D, f = F;
   const uint32_t bbox = tile_bn(tile) / tile_ctas(tile);
+  p.overlap_prev = p.wait_prev = 1;      // behind what wrote dG and dU
   if (int rc = make_map3(&p.tmA, dG, f, n, 1, f, f * n, 32, 128, false)) return rc;
   if (int rc = make_map3(&p.tmRep[2], dU, f, n, 1, f, f * n, 32, 128, false)) return rc;
   if (int rc = make_map3(&p.tmB, Wg, f, d, 1, f, f * d, 32, bbox, false)) return rc;
@@ -719,7 +730,7 @@ int cu32_gatedFF(const int64_t* s, int length, const float* X, const float* Wg, 
     return thin_product(down, THIN_PLAIN, st);
   }
   if (int rc = gated_tiles(X, Wg, Wu, G, U, H, N, D, F, act, st)) return rc;
-  return product(s, false, true, H, F, Wd, D, Y, N, D, F, work, work_floats, st);
+  return product(s, false, true, H, F, Wd, D, Y, N, D, F, work, work_floats, st, BEHIND);
 }
 
 int cu32_gatedFF_delta(const int64_t* s, int length, const float* dY, const float* X, const float* Wg, const float* Wu,
@@ -736,28 +747,37 @@ int cu32_gatedFF_delta(const int64_t* s, int length, const float* dY, const floa
   // Launches that do not depend on each other stand side by side, so that the tiles of the next fill the last round of
   // the one before: deltaWd with deltaH, and deltaWg with deltaWu.
   if (dWd)
-    if (int rc = product(s, true, true, H, F, dY, D, dWd, F, D, N, work, work_floats, st)) return rc;
+    if (int rc = product(s, true, true, H, F, dY, D, dWd, F, D, N, work, work_floats, st, AFTER)) return rc;
   if (N <= THIN_MAX_ROWS && work && thin_delta_floats(N, D, F) <= work_floats) {
-    const ThinCall h{dY, nullptr, Wd, nullptr, dG, nullptr, dU, G, U, work, N, F, D, act, 0};
+    const ThinCall h{dY, nullptr, Wd, nullptr, dG, nullptr, dU, G, U, work, N, F, D, act, dWd != nullptr};
     if (int rc = thin_product(h, THIN_DELTA, st)) return rc;
     if (dX) {
       const ThinCall x{dG, dU, Wg, Wu, dX, nullptr, nullptr, nullptr, nullptr, work, N, D, F, 0, 1};
       if (int rc = thin_product(x, THIN_DUAL, st)) return rc;
     }
   } else {
-    if (int rc = product(s, false, false, dY, D, Wd, D, dG, N, F, D, work, work_floats, st, dWd != nullptr && dG != H)) return rc;
+    const Order order = dWd == nullptr ? AFTER : dG == H ? BEHIND : BESIDE;
+    if (int rc = product(s, false, false, dY, D, Wd, D, dG, N, F, D, work, work_floats, st, order)) return rc;
     const long long vecs = static_cast<long long>(N) * F / 4;
     long long blocks = (vecs + 511) / 512;
     if (blocks > 16LL * device_sm_count()) blocks = 16LL * device_sm_count();
-    gated_delta_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(dG, dU, G, U, vecs, act);
-    if (cudaError_t e = cudaPeekAtLastError()) return static_cast<int>(e);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, gated_delta_kernel, dG, dU, G, U, vecs, act)) return static_cast<int>(e);
     if (dX)
       if (int rc = dual_tiles(s, dG, Wg, dU, Wu, dX, N, D, F, work, work_floats, st)) return rc;
   }
   if (dWg)
-    if (int rc = product(s, true, true, X, D, dG, F, dWg, D, F, N, work, work_floats, st, false)) return rc;
+    if (int rc = product(s, true, true, X, D, dG, F, dWg, D, F, N, work, work_floats, st, BEHIND)) return rc;
   if (dWu)
-    if (int rc = product(s, true, true, X, D, dU, F, dWu, D, F, N, work, work_floats, st, dWg != nullptr)) return rc;
+    if (int rc = product(s, true, true, X, D, dU, F, dWu, D, F, N, work, work_floats, st, dWg ? BESIDE : BEHIND)) return rc;
   return CU32_OK;
 }
 

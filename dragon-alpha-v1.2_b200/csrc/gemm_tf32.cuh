@@ -112,6 +112,8 @@ struct GemmParams {
                         // running (it does not depend on its results - the phases of a strided data gradient)
   int join_prev;        // with overlap_prev: no block leaves before the previous launch has ended, so whoever waits for this
                         // launch has waited for that one too
+  int wait_prev;        // with overlap_prev: this launch does depend on the previous one; only its start-up (barriers, tensor
+                        // memory, descriptors) overlaps that one's end, 2 to 3 us of a short launch
   int sm_reserve;       // SMs the persistent grid leaves free (for a collective's kernels running beside it)
   // im2col geometry (A gathered from an NHWC feature map); unused otherwise.
   // The reduction index runs over (fh, fw, ic) with every filter tap padded to
@@ -442,6 +444,8 @@ __device__ __forceinline__ void gemm_tf32_body(const GemmParams& p) {
   const uint32_t tmem_base = tmem_base_slot;
   // A launch that declared itself independent of this one (GemmParams::overlap_prev) may be scheduled from here on;
   // its CTAs then take over SMs as this grid's CTAs retire, instead of waiting for the whole grid.
+  // (After the wait: a launch beside this one may depend on what this one had to wait for.)
+  if (p.wait_prev) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // CTA 0 times itself in SM cycles and in nanoseconds: summed over launches, cycles / ns is the clock the
   // kernel really ran at (the management library's reading is a coarse sample and can miss short runs).
