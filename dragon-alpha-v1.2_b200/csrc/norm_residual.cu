@@ -35,6 +35,9 @@ constexpr int MAX_WIDTH = 16384;     // floats per row: a cluster of four blocks
 // every row made the kernels wait for it (with four per thread: 145 us forward, 213 us gradients at 8192 x 4096).
 constexpr int VPT = 2;
 constexpr int RING_THREADS = 512;
+// Holds the gradient kernel to 96 registers, without spills (a block has at most RING_THREADS threads; left to itself it takes
+// 118, and one block of 288 threads fills an SM instead of two: 8192 x 2052 rows 89 us instead of 79; elsewhere the same).
+constexpr int DELTA_BOUND = 576;
 
 __device__ __forceinline__ float4 ldg_row(const float* p) {       // read once: not kept in L1
   float4 v;
@@ -419,7 +422,7 @@ struct UnitRows {
 // The ring holds deltaY, R', B and deltaR' of a row.  What the outputs need of a row beside its sums are three values per
 // element, a = deltaR' + q / rms(R'), r^ / rms(R') and b^: they stay in registers over the reduction.
 template <int CL, bool POST, bool GATE>
-__global__ void __launch_bounds__(RING_THREADS) norm_delta_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(DELTA_BOUND) norm_delta_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ __align__(8) RingBars bars;
   __shared__ float slots[2][3][64];
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
 // ------------------------------------------------------------------ host
 // How a row of M floats is laid on a persistent kernel: blocks per row, vectors per block, working threads, and a ring of
 // rows of `arrays` parts that leaves room for the blocks an SM takes.
-constexpr int FORWARD_REGS = 64, DELTA_REGS = 128;      // what the kernels are compiled to at their launch bounds
+constexpr int FORWARD_REGS = 64, DELTA_REGS = 96;      // what the kernels are compiled to at their launch bounds
 struct Shape { int cl, vecs, threads, stages, stage_bytes, slab_bytes, per_sm; };
 
 Shape ring_shape(int M, int arrays, int regs) {
