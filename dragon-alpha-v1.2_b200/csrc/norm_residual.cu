@@ -661,7 +661,7 @@ int cluster_count() {
 // Blocks (clusters) that fill the device once.
 int ring_units(const Shape& s) {
   if (s.cl == 1) return device_sm_count() * s.per_sm;
-  return s.cl == 2 ? cluster_count<2>() : cluster_count<4>();
+  return (s.cl == 2 ? cluster_count<2>() : cluster_count<4>()) * s.per_sm;
 }
 
 template <void (*kernel)(NormParams)>
