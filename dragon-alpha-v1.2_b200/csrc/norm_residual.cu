@@ -620,8 +620,10 @@ Shape ring_shape(int M, int arrays, int regs) {
   s.threads = ((s.vecs + VPT - 1) / VPT + 31) / 32 * 32;
   s.slab_bytes = s.vecs * 16;
   s.stage_bytes = (s.slab_bytes * arrays + 127) / 128 * 128;
-  // blocks per SM: by shared memory at three rows each, by the registers per thread
-  const int by_smem = 220 * 1024 / (3 * s.stage_bytes + 2048), by_regs = 65536 / (regs * s.threads);
+  // Blocks per SM: by shared memory and by the registers per thread.  Three rows in a ring, but two in a cluster's, whose
+  // exchange of sums a second block covers better than a third row (gradients of 8192 x 5000: 161 us, with three 213;
+  // single blocks of 256 columns: 52 us with three, 63 with two).
+  const int rows = s.cl == 1 ? 3 : 2, by_smem = 220 * 1024 / (rows * s.stage_bytes + 2048), by_regs = 65536 / (regs * s.threads);
   s.per_sm = by_smem < by_regs ? by_smem : by_regs;
   if (s.per_sm < 1) s.per_sm = 1;
   s.stages = (220 * 1024 / s.per_sm - 2048) / s.stage_bytes;
