@@ -24,7 +24,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CUFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 
 CU_SOURCES = ["cu32_api.cu", "gemm_kk.cu", "gemm_kk_softmax.cu", "gemm_rep.cu", "gemm_kn.cu", "gemm_nn.cu", "gemm_nn_im2col.cu",
-              "gemm_gated.cu", "gemm_dual.cu", "gemm_thin.cu", "gated_ff.cu", "norm_residual.cu", "grad_clip.cu"]
+              "gemm_gated.cu", "gemm_dual.cu", "gemm_thin.cu", "gated_outer.cu", "gated_ff.cu", "norm_residual.cu", "grad_clip.cu"]
 CPP_SOURCES = ["jni_exports.cpp"]
 HEADERS = ["sm100_ptx.cuh", "gemm_tf32.cuh", "gated_act.cuh", "gated_thin.h", "gemm_launch.h", "cu32_host.h", "jni_min.h", "../../include/dragon_cu32.h",
            "../../include/dragon_cuda.h"]

@@ -10,7 +10,7 @@
 //   issue slots beyond: 16 rows would take as long as two calls.
 // Up to 128 rows: the same reading bounds it, but the products run on the tensor cores with the weights as the tile's
 //   rows (gemm_thin.cu; 16 rows 117 us, 128 rows 251 us, where the tiles below take 315 and 320 us); it needs scratch.
-//   The gradients use it from one row on.
+//   The gradients use it from one row on, with all weight gradients in one launch up to 24 rows (gated_outer.cu).
 // More rows: the contraction kernel (gemm_tf32.cuh) with both projections in one launch and act(G) * U formed in the
 //   registers that hold the sums, and with the two products of deltaX in one accumulation.  6 N D F flop forward and
 //   12 N D F backward at the FP32-accurate rate bound it.
@@ -745,18 +745,24 @@ int cu32_gatedFF_delta(const int64_t* s, int length, const float* dY, const floa
   if (int rc = check_dims(N, D, F, act)) return rc;
   if (!all_aligned16(dY, X, Wg, Wu, Wd, G, U, H, dG, dU, dX, dWg, dWu, dWd, work)) return CU32_E_ALIGN;
   // Launches that do not depend on each other stand side by side, so that the tiles of the next fill the last round of
-  // the one before: deltaWd with deltaH, and deltaWg with deltaWu.
-  if (dWd)
+  // the one before: deltaWd with deltaH, and deltaWg with deltaWu.  With few rows all three are one launch at the end
+  // (deltaWd, which reads H, before the others where deltaG replaces H).
+  const bool outer = N <= OUTER_MAX_ROWS, first = dWd && (!outer || dG == H);
+  const OuterPair of_down{H, dY, dWd, F, D};
+  if (first && outer) {
+    if (int rc = outer_products(&of_down, 1, N, false, st)) return rc;
+  } else if (first) {
     if (int rc = product(s, true, true, H, F, dY, D, dWd, F, D, N, work, work_floats, st, AFTER)) return rc;
+  }
   if (N <= THIN_MAX_ROWS && work && thin_delta_floats(N, D, F) <= work_floats) {
-    const ThinCall h{dY, nullptr, Wd, nullptr, dG, nullptr, dU, G, U, work, N, F, D, act, dWd != nullptr};
+    const ThinCall h{dY, nullptr, Wd, nullptr, dG, nullptr, dU, G, U, work, N, F, D, act, first};
     if (int rc = thin_product(h, THIN_DELTA, st)) return rc;
     if (dX) {
       const ThinCall x{dG, dU, Wg, Wu, dX, nullptr, nullptr, nullptr, nullptr, work, N, D, F, 0, 1};
       if (int rc = thin_product(x, THIN_DUAL, st)) return rc;
     }
   } else {
-    const Order order = dWd == nullptr ? AFTER : dG == H ? BEHIND : BESIDE;
+    const Order order = !first ? AFTER : dG == H ? BEHIND : BESIDE;
     if (int rc = product(s, false, false, dY, D, Wd, D, dG, N, F, D, work, work_floats, st, order)) return rc;
     const long long vecs = static_cast<long long>(N) * F / 4;
     long long blocks = (vecs + 511) / 512;
@@ -773,6 +779,14 @@ int cu32_gatedFF_delta(const int64_t* s, int length, const float* dY, const floa
     if (cudaError_t e = cudaLaunchKernelEx(&cfg, gated_delta_kernel, dG, dU, G, U, vecs, act)) return static_cast<int>(e);
     if (dX)
       if (int rc = dual_tiles(s, dG, Wg, dU, Wu, dX, N, D, F, work, work_floats, st)) return rc;
+  }
+  if (outer) {
+    OuterPair pairs[3];
+    int count = 0;
+    if (dWg) pairs[count++] = OuterPair{X, dG, dWg, D, F};
+    if (dWu) pairs[count++] = OuterPair{X, dU, dWu, D, F};
+    if (dWd && !first) pairs[count++] = of_down;
+    return count > 0 ? outer_products(pairs, count, N, true, st) : CU32_OK;
   }
   if (dWg)
     if (int rc = product(s, true, true, X, D, dG, F, dWg, D, F, N, work, work_floats, st, BEHIND)) return rc;

@@ -1,4 +1,5 @@
-// Products of up to 128 rows with a large weight (gemm_thin.cu).
+// Products of the gated block with few rows: with a large weight (gemm_thin.cu), and the weights' gradients
+// (gated_outer.cu).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -22,5 +23,14 @@ struct ThinCall {
 };
 long long thin_work_floats(int N, int M, int K, ThinForm form);
 int thin_product(const ThinCall& c, ThinForm form, cudaStream_t st);
+
+// out[M, N] = A[K, M]^T B[K, N], M and N multiples of 4
+struct OuterPair {
+  const float* A; const float* B; float* out;
+  int M, N;
+};
+constexpr int OUTER_MAX_ROWS = 24;
+// Up to three of them in one launch; behind: the launch before is of the same call.
+int outer_products(const OuterPair* pairs, int count, int K, bool behind, cudaStream_t st);
 
 }  // namespace dragon

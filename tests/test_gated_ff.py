@@ -427,3 +427,46 @@ def test_gradients_of_rows_do_not_depend_on_their_company_with_scratch(pkg, cuda
         for n, was in clean.items():
             now = b.get(torch, n)
             assert not torch.isfinite(now[rows // 2]).any() and torch.equal(now[others], was[others]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 7, 24, 25])
+@pytest.mark.parametrize("dims", [(4, 4), (60, 260), (68, 1028), (260, 64), (1500, 1284)], ids=str)
+def test_weight_gradients_of_few_rows(pkg, cuda, rows, dims):
+    """Edges of the few-row weight gradients' tiles (64 x 256 and multiples), with and without scratch, deltaG over H."""
+    torch = cuda
+    D, F = dims
+    b = Block(torch, rows, D, F, seed=rows)
+    work = torch.empty(pkg.cu32.Cuda_gatedFF.work(rows, D, F) + 4, device="cuda")
+    b.forward(pkg, 0, work=work)
+    G, U, H = (b.get(torch, n) for n in "GUH")
+    for w in (work, None):
+        b.backward(pkg, 0, work=w)
+        check_backward(torch, b, 0, G, U)
+    kept = {n: b.get(torch, n) for n in ("dG", "dU", "dWg", "dWu", "dWd")}
+    b.backward(pkg, 0, work=None, over="U")            # deltaG over H, deltaU over U: deltaWd has to read H before
+    assert torch.equal(b.get(torch, "H"), kept["dG"]) and torch.equal(b.get(torch, "U"), kept["dU"])
+    for n in ("dWg", "dWu", "dWd"):
+        assert torch.equal(b.get(torch, n), kept[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wanted", [("dWg",), ("dWu",), ("dWd",), ("dWd", "dWu"), ("dX", "dWd"), ()], ids=str)
+def test_few_rows_single_gradients(pkg, cuda, wanted):
+    import gpu_util as Gu
+    torch = cuda
+    N, D, F = 6, 68, 132
+    b = Block(torch, N, D, F, seed=77)
+    work = torch.empty(pkg.cu32.Cuda_gatedFF.work(N, D, F) + 4, device="cuda")
+    b.forward(pkg, 0, work=work)
+    b.backward(pkg, 0, work=work)
+    all_of = {n: b.get(torch, n) for n in ("dX", "dWg", "dWu", "dWd", "dG", "dU")}
+    for n in ("dX", "dWg", "dWu", "dWd", "dG", "dU"):
+        getattr(b, n).view.fill_(-7.0)
+    o = lambda n: getattr(b, n).ptr if n in wanted else 0  # noqa: E731
+    pkg.cu32.Cuda_gatedFF.gatedFF_delta(
+        [Gu.stream()], 1, b.dY.data_ptr(), b.X.data_ptr(), b.Wg.data_ptr(), b.Wu.data_ptr(), b.Wd.data_ptr(), b.G.ptr, b.U.ptr,
+        b.H.ptr, b.dG.ptr, b.dU.ptr, o("dX"), o("dWg"), o("dWu"), o("dWd"), work.data_ptr(), work.numel(), N, D, F, 0)
+    for n, was in all_of.items():
+        now = b.get(torch, n)
+        assert torch.equal(now, was) if n in wanted or n in ("dG", "dU") else bool((now == -7.0).all()), n
