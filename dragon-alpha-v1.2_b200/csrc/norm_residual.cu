@@ -57,6 +57,15 @@ __device__ __forceinline__ float4 clip4(float4 v, int col, int width) {
   return v;
 }
 
+// On the way out they are 0 as long as the row's factors are finite; else 0 * NaN is put right behind the vector stores, by the
+// threads that made them.
+__device__ __forceinline__ bool all_finite(float sum_of_factors) { return fabsf(sum_of_factors) <= 3.4e38f; }
+__device__ __forceinline__ void clear_padding(float* part, int vec0, int vecs, int width) {
+  for (int v = threadIdx.x; v < vecs; v += blockDim.x)
+    for (int j = 0; j < 4; ++j)
+      if ((vec0 + v) * 4 + j >= width) part[v * 4 + j] = 0.0f;
+}
+
 __device__ __forceinline__ float4 ones4() { return make_float4(1.f, 1.f, 1.f, 1.f); }
 __device__ __forceinline__ float square_sum(float4 v) { return v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w; }
 __device__ __forceinline__ float4 scaled(float4 v, float f, float4 w) {
@@ -213,6 +222,10 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const __grid_constan
   for (int i = 0; i < V; ++i) {
     const int v = i * blockDim.x + threadIdx.x;
     if (v < vecs) *reinterpret_cast<float4*>(p.Y + base + v * 4) = scaled(r[i], rr, load_weight(p.wpre, v, p.width));
+  }
+  if (!all_finite(rb + rr + p.scale + p.res_scale)) {
+    clear_padding(p.Rout + base, 0, vecs, p.width);
+    clear_padding(p.Y + base, 0, vecs, p.width);
   }
 }
 
@@ -385,6 +398,10 @@ __global__ void __launch_bounds__(RING_THREADS, 2) norm_forward_ring_kernel(cons
       const int v = i * T + threadIdx.x;
       if (v < vecs) *reinterpret_cast<float4*>(p.Y + base + v * 4) = scaled(r[i], rr, wpre[i]);
     }
+    if (!all_finite(rb + rr + p.scale + p.res_scale)) {
+      clear_padding(p.Rout + base, vec0, vecs, p.width);
+      clear_padding(p.Y + base, vec0, vecs, p.width);
+    }
     ask_gate(row + p.units);
   }
   if (lost) {
@@ -536,7 +553,7 @@ __global__ void __launch_bounds__(DELTA_BOUND) norm_delta_kernel(const __grid_co
         one(a[i].y, c[i].y, b[i].y, gate[i].y, wpost[i].y, odr.y, odb.y, dwpost[i].y, dgate[i].y);
         one(a[i].z, c[i].z, b[i].z, gate[i].z, wpost[i].z, odr.z, odb.z, dwpost[i].z, dgate[i].z);
         one(a[i].w, c[i].w, b[i].w, gate[i].w, wpost[i].w, odr.w, odb.w, dwpost[i].w, dgate[i].w);
-        *reinterpret_cast<float4*>(p.dR + base + v * 4) = odr;     // padding columns: every operand was cleared
+        *reinterpret_cast<float4*>(p.dR + base + v * 4) = odr;     // padding columns: the column sums' kernel clears them
         *reinterpret_cast<float4*>(p.dB + base + v * 4) = odb;
       }
     }
@@ -544,7 +561,9 @@ __global__ void __launch_bounds__(DELTA_BOUND) norm_delta_kernel(const __grid_co
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int v = i * T + threadIdx.x;
-        if (v < vecs) *reinterpret_cast<float4*>(p.dgate + static_cast<long long>(group) * p.M + (vec0 + v) * 4) = dgate[i];
+        if (v < vecs)
+          *reinterpret_cast<float4*>(p.dgate + static_cast<long long>(group) * p.M + (vec0 + v) * 4) =
+              clip4(dgate[i], (vec0 + v) * 4, p.width);
         dgate[i] = zero4();
       }
     }
@@ -574,19 +593,32 @@ struct ColSumParams {
   const float* in[3];
   float* out[3];
   int rows[3];      // partial rows per output row
-  int M;
+  int M, width, N, groups;
+  float* rows_out[2];    // deltaR, deltaB: columns >= width are set to zeros here, because a row whose sums are not finite
+                         // leaves NaN there (looking at it in the rows' kernel cost wide rows 5 to 10 % of its time)
 };
 // Block: 8 vectors of columns x 32 slices of the rows; blockIdx.y = output row, blockIdx.z = which sum.
 __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ ColSumParams p) {
   __shared__ float4 part[32][8];
   const int z = blockIdx.z;
   const float* in = p.in[z];
-  if (in == nullptr || (z < 2 && blockIdx.y > 0)) return;
+  const bool sums = in != nullptr && static_cast<int>(blockIdx.y) < (z < 2 ? 1 : p.groups);
+  if (!sums && z > 0) return;
   const int c = threadIdx.x & 7, slice = threadIdx.x >> 3;
   const int v = blockIdx.x * 8 + c;
   const int rows = p.rows[z];
   float4 s = zero4();
   asm volatile("griddepcontrol.wait;" ::: "memory");      // the partial rows are complete
+  if (z == 0 && p.width < p.M) {
+    const int warps = gridDim.x * gridDim.y * 8, warp = (blockIdx.y * gridDim.x + blockIdx.x) * 8 + (threadIdx.x >> 5);
+    for (int row = warp; row < p.N; row += warps)
+      for (int col = p.width + (threadIdx.x & 31); col < p.M; col += 32) {
+        const long long at = static_cast<long long>(row) * p.M + col;
+        p.rows_out[0][at] = 0.0f;
+        p.rows_out[1][at] = 0.0f;
+      }
+  }
+  if (!sums) return;
   if (v < p.M / 4) {
     const float4* src = reinterpret_cast<const float4*>(in) + static_cast<long long>(blockIdx.y) * rows * (p.M / 4) + v;
 #pragma unroll 4
@@ -602,7 +634,7 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
       const float4 x = part[k][c];
       s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
     }
-    reinterpret_cast<float4*>(p.out[z])[static_cast<long long>(blockIdx.y) * (p.M / 4) + v] = s;
+    reinterpret_cast<float4*>(p.out[z])[static_cast<long long>(blockIdx.y) * (p.M / 4) + v] = clip4(s, v * 4, p.width);
   }
 }
 
@@ -816,12 +848,22 @@ int cu32_normResidual_delta(int64_t stream, const float* dRout, const float* dY,
   else e = launch_delta<4>(wpost != nullptr, gate != nullptr, s, p, st);
   if (e != cudaSuccess) return static_cast<int>(e);
   ColSumParams c{};
-  c.M = M;
+  c.M = M; c.width = width; c.N = N;
+  c.rows_out[0] = dR; c.rows_out[1] = dB;
   c.in[0] = p.part_pre; c.out[0] = dwpre; c.rows[0] = r.units;
   if (wpost) { c.in[1] = p.part_post; c.out[1] = dwpost; c.rows[1] = r.units; }
   const bool gate_sum = gate && !r.direct;
   if (gate_sum) { c.in[2] = p.part_gate; c.out[2] = dgate; c.rows[2] = r.chunks; }
-  const dim3 grid(static_cast<unsigned>((M / 4 + 7) / 8), gate_sum ? static_cast<unsigned>(r.groups) : 1u, gate_sum ? 3u : 2u);
+  c.groups = r.groups;
+  const int across = (M / 4 + 7) / 8;
+  int down = gate_sum ? r.groups : 1;
+  if (width < M) {      // a warp clears some 16 rows
+    int clear = (N / 128 + across - 1) / across;
+    const int most = 8 * device_sm_count() / across;
+    if (clear > most) clear = most;
+    if (down < clear) down = clear;
+  }
+  const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(down), gate_sum ? 3u : 2u);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(256, 1, 1);

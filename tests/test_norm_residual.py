@@ -313,3 +313,42 @@ def test_norm_in_a_graph_and_on_two_streams(pkg, cuda):
     check_forward(torch, c)
     check_backward(torch, c)
     del graph
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [20, 700])
+@pytest.mark.parametrize("width", [130, 4097])
+@pytest.mark.parametrize("gate_rows", [1, 9, 700])
+def test_norm_padding_is_zero_beside_bad_rows(pkg, cuda, N, width, gate_rows):
+    """Columns >= width of every output are zeros also where the row's sums are NaN or infinite (out() looks at them)."""
+    torch = cuda
+    c = Case(torch, N, width, gate_rows, True, seed=61, pad=4)
+    work = c.scratch(torch, pkg)
+    c.forward(pkg)
+    c.backward(pkg, work)
+    clean = {n: c.out(torch, n) for n in ("Rout", "Y", "dR", "dB")}
+    c.B[5, 7] = float("nan")
+    c.R[9, 1] = float("inf")
+    c.dY[12, 3] = float("-inf")
+    c.forward(pkg)
+    c.backward(pkg, work)
+    others = [i for i in range(N) if i not in (5, 9, 12)]
+    for n, was in clean.items():
+        now = c.out(torch, n)
+        assert torch.equal(now[others], was[others]), n
+    for n in ("dgate", "dwpost", "dwpre"):
+        c.out(torch, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3000, 5000, 0), (3000, 2052, 300), (1200, 10000, 75), (20000, 260, 1700), (9000, 1536, 2500),
+                                   (700, 16384, 70)], ids=str)
+def test_norm_many_rows_per_block(pkg, cuda, shape):
+    """Rings that go round many times: single blocks, clusters of two and four, two clusters to an SM."""
+    torch = cuda
+    N, width, gate_rows = shape
+    c = Case(torch, N, width, gate_rows, True, seed=62)
+    c.forward(pkg)
+    check_forward(torch, c)
+    c.backward(pkg, c.scratch(torch, pkg))
+    check_backward(torch, c)
