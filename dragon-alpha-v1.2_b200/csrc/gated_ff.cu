@@ -685,6 +685,25 @@ bool any_null(const P*... p) { return (... || (p == nullptr)); }
 template <class... P>
 bool all_aligned16(const P*... p) { return (... && aligned16(p)); }
 
+// An array of a call; null where the call neither reads nor writes it.
+struct Span { const float* p; long long n; };
+inline bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.p && b.p && x < y + 4ull * static_cast<unsigned long long>(b.n) && y < x + 4ull * static_cast<unsigned long long>(a.n);
+}
+// Whether an output lies over an operand or another output.  Which of them would still come out right depends on the form a
+// call takes, and so on the number of rows: all are refused.
+template <int OUTS, int INS>
+bool outputs_overlap(const Span (&out)[OUTS], const Span (&in)[INS]) {
+  for (int i = 0; i < OUTS; ++i) {
+    for (int j = 0; j < INS; ++j)
+      if (overlap(out[i], in[j])) return true;
+    for (int j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return true;
+  }
+  return false;
+}
+
 }  // namespace
 }  // namespace dragon
 
@@ -717,6 +736,8 @@ int cu32_gatedFF(const int64_t* s, int length, const float* X, const float* Wg, 
   if (any_null(X, Wg, Wu, Wd, H, Y) || (G == nullptr) != (U == nullptr)) return CU32_E_NULL;
   if (int rc = check_dims(N, D, F, act)) return rc;
   if (!all_aligned16(X, Wg, Wu, Wd, G, U, H, Y, work)) return CU32_E_ALIGN;
+  const long long nd = static_cast<long long>(N) * D, nf = static_cast<long long>(N) * F, df = static_cast<long long>(D) * F;
+  if (outputs_overlap({{G, nf}, {U, nf}, {H, nf}, {Y, nd}}, {{X, nd}, {Wg, df}, {Wu, df}, {Wd, df}})) return CU32_E_ARG;
   if (N <= ROWS_MAX) {
     const RowsCall up{X, Wg, Wu, H, G, U, N, F, D, act, 0};
     if (int rc = rows_any<2>(up, st)) return rc;
@@ -744,6 +765,13 @@ int cu32_gatedFF_delta(const int64_t* s, int length, const float* dY, const floa
   if ((dX && any_null(Wg, Wu)) || ((dWg || dWu) && !X) || (dWd && !H)) return CU32_E_NULL;
   if (int rc = check_dims(N, D, F, act)) return rc;
   if (!all_aligned16(dY, X, Wg, Wu, Wd, G, U, H, dG, dU, dX, dWg, dWu, dWd, work)) return CU32_E_ALIGN;
+  const long long nd = static_cast<long long>(N) * D, nf = static_cast<long long>(N) * F, df = static_cast<long long>(D) * F;
+  const float* const x = dWg || dWu ? X : nullptr;      // operands that only some of the gradients need
+  const float* const h = dWd && H != dG ? H : nullptr;  // and those that are replaced
+  const float *const g = G != dU ? G : nullptr, *const u = U != dU ? U : nullptr;
+  if (outputs_overlap({{dG, nf}, {dU, nf}, {dX, nd}, {dWg, df}, {dWu, df}, {dWd, df}},
+                      {{dY, nd}, {x, nd}, {dX ? Wg : nullptr, df}, {dX ? Wu : nullptr, df}, {Wd, df}, {g, nf}, {u, nf}, {h, nf}}))
+    return CU32_E_ARG;
   // Launches that do not depend on each other stand side by side, so that the tiles of the next fill the last round of
   // the one before: deltaWd with deltaH, and deltaWg with deltaWu.  With few rows all three are one launch at the end
   // (deltaWd, which reads H, before the others where deltaG replaces H).

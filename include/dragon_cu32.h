@@ -441,7 +441,8 @@ CU32_API int cu32_batchMatMulT2_softmax(const int64_t* streams, int length, cons
  *   deltaG may be H, which are then replaced (deltaG must not be G, U or deltaU: CU32_E_ARG).  deltaX = deltaG Wg^T +
  *   deltaU Wu^T, deltaWg = X^T deltaG, deltaWu = X^T deltaU, deltaWd = H^T deltaY.  deltaX, deltaWg, deltaWu and deltaWd
  *   may each be null: that gradient is not computed (and the operands only it needs may be null).
- * Apart from these replacements no output may overlap an operand or another output.
+ * Apart from these replacements no output may overlap an operand that the call reads or another output (CU32_E_ARG), nor
+ * the scratch.
  * work: work_floats floats of scratch for partial sums, or null / 0 (slower); its contents mean nothing between calls.
  *   Calls that may overlap, and graphs that may be replayed side by side, need scratch of their own.  cu32_gatedFF_work
  *   says how many floats the two calls can use; with fewer they give correct results more slowly.

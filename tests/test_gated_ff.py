@@ -151,6 +151,40 @@ def test_gated_ff_refusals(pkg):
         pkg.cu32.Cuda_gatedFF.gatedFF([0], 1, 0, P, P, P, 0, 0, P, P, 0, 0, 4, 8, 12, 0)
 
 
+def test_gated_ff_refuses_overlaps(pkg):
+    """An output over an operand or another output, whole or in part: CU32_E_ARG, apart from the replacements the calls
+    allow.  (With up to 24 rows deltaU over H would leave deltaWd without its H, and deltaX over deltaY without its deltaY.)"""
+    lib = pkg.cu32.load()
+    s = (ctypes.c_int64 * 10)()
+    for N, D, F in ((4, 8, 12), (40, 8, 12), (300, 8, 12)):
+        size = {"X": N * D, "Y": N * D, "dY": N * D, "dX": N * D, "Wg": D * F, "Wu": D * F, "Wd": D * F, "dWg": D * F,
+                "dWu": D * F, "dWd": D * F, "G": N * F, "U": N * F, "H": N * F, "dG": N * F, "dU": N * F}
+        place, at = {}, 0x10000
+        for name, n in size.items():            # one behind the other, without a gap
+            place[name] = at
+            at += 4 * n
+
+        def fwd(**at):
+            a = dict(place, **at)
+            return lib.cu32_gatedFF(s, 1, a["X"], a["Wg"], a["Wu"], a["Wd"], a["G"], a["U"], a["H"], a["Y"], 0, 0, N, D, F, 0)
+
+        def bwd(**at):
+            a = dict(place, **at)
+            return lib.cu32_gatedFF_delta(s, 1, *(a[n] for n in ("dY", "X", "Wg", "Wu", "Wd", "G", "U", "H", "dG", "dU", "dX", "dWg",
+                                                                 "dWu", "dWd")), 0, 0, N, D, F, 0)
+        for call, outs, ins, allowed in ((fwd, ("G", "U", "H", "Y"), ("X", "Wg", "Wu", "Wd"), ()),
+                                         (bwd, ("dG", "dU", "dX", "dWg", "dWu", "dWd"), ("dY", "X", "Wg", "Wu", "Wd", "G", "U", "H"),
+                                          (("dG", "H"), ("dU", "G"), ("dU", "U")))):
+            for out in outs:
+                for other in outs + ins:
+                    if other == out:
+                        continue
+                    for there in (place[other], place[other] + 4 * size[other] - 16, place[other] - 4 * size[out] + 16):
+                        if there == place[other] and (out, other) in allowed:
+                            continue
+                        assert call(**{out: there}) == -8, (N, out, other)
+
+
 # ---------------------------------------------------------------------------------------------------- on the GPU
 SHAPES = [
     # N, D, F: up to 8 rows, up to 128 rows (both: one kernel per power of two), tiles; with every kind of tail
@@ -470,3 +504,23 @@ def test_few_rows_single_gradients(pkg, cuda, wanted):
     for n, was in all_of.items():
         now = b.get(torch, n)
         assert torch.equal(now, was) if n in wanted or n in ("dG", "dU") else bool((now == -7.0).all()), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [6, 40, 200])
+def test_delta_over_what_the_call_does_not_read(pkg, cuda, rows):
+    """Without deltaWd nothing reads H, without the weights' gradients nothing reads X: they may be replaced."""
+    import gpu_util as Gu
+    torch = cuda
+    D, F = 68, 132
+    b = Block(torch, rows, D, F, seed=78)
+    work = torch.empty(pkg.cu32.Cuda_gatedFF.work(rows, D, F) + 4, device="cuda")
+    b.forward(pkg, 0, work=work)
+    b.backward(pkg, 0, work=work)
+    want = {n: b.get(torch, n) for n in ("dX", "dG", "dU")}
+    b.dG.view.fill_(float("nan"))
+    pkg.cu32.Cuda_gatedFF.gatedFF_delta(
+        [Gu.stream()], 1, b.dY.data_ptr(), b.X.data_ptr(), b.Wg.data_ptr(), b.Wu.data_ptr(), b.Wd.data_ptr(), b.G.ptr, b.U.ptr,
+        b.H.ptr, b.dG.ptr, b.H.ptr, b.X.data_ptr(), 0, 0, 0, work.data_ptr(), work.numel(), rows, D, F, 0)
+    assert torch.equal(b.get(torch, "dG"), want["dG"]) and torch.equal(b.get(torch, "H"), want["dU"])
+    assert torch.equal(b.X, want["dX"])
