@@ -35,6 +35,7 @@ static std::atomic<int> g_rep_lazy{1};
 static std::atomic<int> g_ring_paired{1};
 static std::atomic<int> g_ring_fixed{1};
 static std::atomic<int> g_phase_fused{1};
+static std::atomic<int> g_rows_give_up{0};
 
 void load_env_once() {
   static std::once_flag once;
@@ -166,6 +167,7 @@ static int pick_tile(long long M, int N, long long z) {
 // configuration's balanced default.
 // Also sets how many chunks are summed in registers between flushes to memory: 256 k-blocks (K = 8192).
 int forced_tile() { return g_tile.load(); }
+int rows_give_up() { return g_rows_give_up.load(); }
 void choose_rings(GemmParams* p) {
   p->flush_chunks = 256 / p->kc > 1 ? 256 / p->kc : 1;
   p->ring_raw = g_ring_raw.load();
@@ -1467,6 +1469,7 @@ int cu32_tune(const char* key, int value) {
   if (!std::strcmp(key, "ring_paired")) { g_ring_paired = value ? 1 : 0; return CU32_OK; }
   if (!std::strcmp(key, "ring_fixed")) { g_ring_fixed = value ? 1 : 0; return CU32_OK; }
   if (!std::strcmp(key, "phase_fused")) { g_phase_fused = value ? 1 : 0; return CU32_OK; }
+  if (!std::strcmp(key, "rows_give_up")) { if (value < 0 || value > 16) return CU32_E_ARG; g_rows_give_up = value; return CU32_OK; }
   if (!std::strcmp(key, "sm_reserve")) { if (value < 0 || value > 1024) return CU32_E_ARG; g_sm_reserve = value; return CU32_OK; }
   return CU32_E_ARG;
 }
@@ -1488,6 +1491,7 @@ int cu32_get_tune(const char* key, int* value) {
   if (!std::strcmp(key, "ring_paired")) { *value = g_ring_paired; return CU32_OK; }
   if (!std::strcmp(key, "ring_fixed")) { *value = g_ring_fixed; return CU32_OK; }
   if (!std::strcmp(key, "phase_fused")) { *value = g_phase_fused; return CU32_OK; }
+  if (!std::strcmp(key, "rows_give_up")) { *value = g_rows_give_up; return CU32_OK; }
   if (!std::strcmp(key, "sm_reserve")) { *value = g_sm_reserve; return CU32_OK; }
   if (!std::strcmp(key, "last_tile")) { *value = g_last_tile; return CU32_OK; }
   return CU32_E_ARG;

@@ -34,6 +34,8 @@ struct RowsParams {
   int N, M, act;
   int ktiles, items, clusters, stages;
   int early;                  // the grid may start before the one that writes X has ended
+  int give_up;                // tests: w + 1, or ROWS_WARPS + w + 1: worker warp w of block 0 loses its first wait for a tile,
+                              // or for an item's sums; 0: none
   int* status;
 };
 
@@ -106,13 +108,13 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_cons
   using Cfg = RowsCfg<NR, MATS, CPW, S>;
   extern __shared__ __align__(128) uint8_t rows_smem[];
   __shared__ __align__(8) uint64_t bar_full[ROWS_MAX_STAGES], bar_empty[ROWS_MAX_STAGES], bar_box[2];
-  __shared__ volatile int abort_flag;
+  __shared__ volatile int abort_flag, lost[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = S > 1 ? cluster_ctarank() : 0u;
   const uint32_t ring = (smem_u32(rows_smem) + 127u) & ~127u;
   const uint32_t red = ring + Cfg::STAGES * Cfg::TILE_BYTES, box = red + Cfg::RED_BYTES;
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    abort_flag = lost[0] = lost[1] = 0;
     for (int i = 0; i < ROWS_MAX_STAGES; ++i) {
       mbar_init(smem_u32(&bar_full[i]), 1);
       mbar_init(smem_u32(&bar_empty[i]), ROWS_WARPS);
@@ -182,6 +184,11 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_cons
     constexpr int RPL = 4;                 // rows of the tile per lane
     const int k_in = (warp * (32 / LPR) + lane / LPR) * RPL, c_in = (lane % LPR) * 4;
     uint32_t st = 0, ph = 0, done = 0;
+    const int loses = blockIdx.x == 0 ? p.give_up - 1 - warp : -1;
+    // A wait may run out in one warp and succeed in another a moment later.  Whoever lost one says so and goes on to the next
+    // barrier of the workers all the same, behind which all of them look and leave together: nobody waits at a barrier for
+    // warps that have left.  There are two such barriers per item, each with a word of its own, so that a warp that is ahead
+    // says nothing yet where another still has to look.
     bool alive = true;
     for (int item = first_item; alive && item < p.items; item += p.clusters, ++done) {
       f32x2 acc2[NR][MATS][2];
@@ -215,13 +222,13 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_cons
             }
           }
       };
-      auto arrived = [&](int t) {
-        if (mbar_wait(smem_u32(&bar_full[st]), ph, &abort_flag)) return true;
+      auto arrived = [&](int t, bool loses_it) {
+        if (!loses_it && mbar_wait(smem_u32(&bar_full[st]), ph, &abort_flag)) return true;
         if (lane == 0) give_up(ROLE_ROWS_TILE, t);
         return false;
       };
       Part a, b;
-      alive = arrived(t0);
+      alive = arrived(t0, loses == 0);
       if (alive) load(a, ring + st * Cfg::TILE_BYTES, 0);
       for (int t = t0; alive && t < t1; ++t) {
         load(b, ring + st * Cfg::TILE_BYTES, JB);
@@ -230,12 +237,16 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_cons
         if (++st == Cfg::STAGES) { st = 0; ph ^= 1u; }
         multiply(a);
         if (t + 1 < t1) {
-          alive = arrived(t + 1);
+          alive = arrived(t + 1, false);
           if (alive) load(a, ring + st * Cfg::TILE_BYTES, 0);
         }
         multiply(b);
       }
-      if (!alive) break;
+      if (!alive) {
+        lost[0] = 1;
+        workers_sync();
+        break;
+      }
       float acc[NR][MATS][4];
 #pragma unroll
       for (int n = 0; n < NR; ++n)
@@ -270,6 +281,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_cons
                      make_float4(acc[g + n][m][0], acc[g + n][m][1], acc[g + n][m][2], acc[g + n][m][3]));
         }
         workers_sync();
+        if (g == 0 && lost[0]) {
+          alive = false;
+          break;
+        }
         for (int e = threadIdx.x; e < Cfg::GROUP * MATS * CV; e += ROWS_WORKERS) {
           float4 v = lds_v4(red + e * 16);
 #pragma unroll
@@ -286,8 +301,11 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_cons
         }
         workers_sync();
       }
-      if (!mbar_wait(smem_u32(&bar_box[par]), (done >> 1) & 1u, &abort_flag)) {
+      if (!alive) break;
+      if (loses == ROWS_WARPS || !mbar_wait(smem_u32(&bar_box[par]), (done >> 1) & 1u, &abort_flag)) {
         if (lane == 0) give_up(ROLE_ROWS_SUM, item);
+        lost[1] = 1;
+        workers_sync();
         break;
       }
       for (int e = threadIdx.x; e < NR * OV; e += ROWS_WORKERS) {
@@ -317,9 +335,15 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_cons
         }
       }
       workers_sync();                        // the inbox has been read before this block sends its next item
+      if (lost[1]) break;
     }
   }
   __syncthreads();
+  if (abort_flag) {                          // what is on its way, here or from here to others, lands first: 0.1 ms
+    const long long c0 = clock64();
+    while (clock64() - c0 < 200000LL) {
+    }
+  }
   if (S > 1) cluster_sync();                 // nobody leaves while a block may still send to it
 }
 
@@ -375,7 +399,7 @@ int rows_launch(const RowsCall& c, cudaStream_t st) {
     if (int rc = make_map_rows(&p.tmW[1], c.W1, c.M, c.K, CPW, Cfg::KT)) return rc;
   if (int rc = make_map_rows(&p.tmX, c.X, c.K, c.N, Cfg::KT, NR)) return rc;
   p.out = c.out; p.G = c.G; p.U = c.U;
-  p.N = c.N; p.M = c.M; p.act = c.act; p.early = c.early;
+  p.N = c.N; p.M = c.M; p.act = c.act; p.early = c.early; p.give_up = rows_give_up();
   p.ktiles = (c.K + Cfg::KT - 1) / Cfg::KT;
   p.items = (c.M + CPW - 1) / CPW;
   cudaError_t e = rows_clusters<NR, MATS, CPW, S>(&p.clusters);

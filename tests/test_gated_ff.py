@@ -524,3 +524,34 @@ def test_delta_over_what_the_call_does_not_read(pkg, cuda, rows):
         b.H.ptr, b.dG.ptr, b.H.ptr, b.X.data_ptr(), 0, 0, 0, work.data_ptr(), work.numel(), rows, D, F, 0)
     assert torch.equal(b.get(torch, "dG"), want["dG"]) and torch.equal(b.get(torch, "H"), want["dU"])
     assert torch.equal(b.X, want["dX"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,keys", [((3, 64, 20000), (1, 6, 9, 15)), ((8, 64, 132), (3, 12)), ((1, 260, 64), (8, 9))], ids=str)
+def test_a_lost_wait_ends_the_call_with_a_status(pkg, cuda, shape, keys):
+    """One warp of a block counts a wait as run out while the others of its block, and of its cluster (one, two and four
+    blocks), got theirs: the kernels end, the status word names a role of theirs, nothing is written beyond the outputs,
+    and the next call is right."""
+    torch = cuda
+    b = Block(torch, *shape, seed=79)
+    try:
+        for key in keys:
+            pkg.cu32.tune("rows_give_up", key)
+            b.forward(pkg, 0)
+            word = pkg.cu32.read_status()
+            assert word >> 24 in (10, 11, 12), hex(word)
+            for name in "GUHY":
+                b.get(torch, name)
+            pkg.cu32.tune("rows_give_up", 0)
+            b.forward(pkg, 0)
+            check_forward(torch, b, 0)
+            assert pkg.cu32.read_status() == 0
+    finally:
+        pkg.cu32.tune("rows_give_up", 0)
+
+
+def test_rows_give_up_key(pkg):
+    lib = pkg.cu32.load()
+    v = ctypes.c_int(-5)
+    assert lib.cu32_get_tune(b"rows_give_up", ctypes.byref(v)) == 0 and v.value == 0
+    assert lib.cu32_tune(b"rows_give_up", 17) == -8 and lib.cu32_tune(b"rows_give_up", -1) == -8
