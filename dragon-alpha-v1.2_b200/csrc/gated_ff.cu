@@ -339,11 +339,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_cons
     }
   }
   __syncthreads();
-  if (abort_flag) {                          // what is on its way, here or from here to others, lands first: 0.1 ms
-    const long long c0 = clock64();
-    while (clock64() - c0 < 200000LL) {
-    }
-  }
+  if (abort_flag) linger();
   if (S > 1) cluster_sync();                 // nobody leaves while a block may still send to it
 }
 

@@ -407,6 +407,7 @@ __global__ void __launch_bounds__(RING_THREADS, 2) norm_forward_ring_kernel(cons
   if (lost) {
     give_up(p, &abort_flag, lost, row);
     if (threadIdx.x == 0) ring.land();
+    if (CL > 1) linger();
   }
   __syncthreads();
   if (CL > 1) cluster_sync();
@@ -573,6 +574,7 @@ __global__ void __launch_bounds__(DELTA_BOUND) norm_delta_kernel(const __grid_co
   if (lost) {
     give_up(p, &abort_flag, lost, row);
     if (threadIdx.x == 0) ring.land();
+    if (CL > 1) linger();
   }
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {

@@ -94,6 +94,14 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity,
   }
 }
 
+// A block that gave up lingers (some 0.1 ms) before it lets its cluster go: what it has sent to the others lands within
+// microseconds, and nobody may have left by then.
+__device__ __forceinline__ void linger() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 200000LL) {
+  }
+}
+
 // ---------------------------------------------------------------- proxies
 // Makes this thread's generic-proxy shared-memory writes visible to the async
 // proxy (TMA, UMMA operand fetch).
