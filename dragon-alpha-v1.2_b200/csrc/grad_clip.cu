@@ -105,40 +105,58 @@ __global__ void __launch_bounds__(THREADS, NORM_BLOCKS_PER_SM) grad_norm_kernel(
 }
 
 // Norm and factor from the partial sums, the same in every thread of the block.
-__device__ __forceinline__ void norm_of(const double* partial, int partials, double max_norm, double* norm, float* factor) {
+__device__ __forceinline__ void norm_of(const double* partial, int partials, double max_norm, double* norm, double* factor) {
   double s = 0.0;
   for (int i = threadIdx.x; i < partials; i += THREADS) s += partial[i];
   *norm = sqrt(block_sum(s));
-  *factor = *norm > max_norm && *norm < INFINITY ? static_cast<float>(max_norm / *norm) : 1.0f;
+  *factor = *norm > max_norm && *norm < INFINITY ? max_norm / *norm : 1.0;
 }
-// result = {norm, factor}, one block
-__global__ void __launch_bounds__(THREADS) grad_result_kernel(const double* partial, int partials, double max_norm, float* result) {
-  double norm;
-  float factor;
+__device__ __forceinline__ void store_result(double norm, double factor, float* result) {
+  result[0] = static_cast<float>(norm);
+  result[1] = static_cast<float>(factor);
+}
+// result = {norm, factor}, and the factor in 64 bits behind the partial sums; one block
+__global__ void __launch_bounds__(THREADS) grad_result_kernel(double* partial, int partials, double max_norm, float* result) {
+  double norm, factor;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   norm_of(partial, partials, max_norm, &norm, &factor);
-  if (threadIdx.x == 0) { result[0] = static_cast<float>(norm); result[1] = factor; }
+  if (threadIdx.x == 0) {
+    store_result(norm, factor, result);
+    partial[partials] = factor;
+  }
 }
 
+// Below the smallest normal FP32 number (2^-126) a factor would lose bits, or all of itself: the products are formed in 64
+// bits there, element by element (norms above 8.5e37 times the limit: not a case to be fast in).
+constexpr double SMALLEST_FACTOR = 1.1754943508222875e-38;
+
 // dst = src * factor.  Where the factor is 1 and a tensor stays in place, nothing is touched.  A norm that is not finite
-// leaves every element as it is (factor 1): the caller sees it in result[0].  partials: 0 when result is there already,
-// else the blocks form it themselves, and the first one writes it.
+// leaves every element as it is (factor 1): the caller sees it in result[0].  direct: the blocks form norm and factor
+// themselves, and the first one writes the result; else the factor lies behind the partial sums.
 template <int CAP>
 __global__ void __launch_bounds__(THREADS, CLIP_BLOCKS_PER_SM) grad_clip_kernel(const __grid_constant__ TensorList<CAP> list,
-                                                                               const double* partial, int partials,
+                                                                               const double* partial, int partials, int direct,
                                                                                double max_norm, float* result) {
-  float factor;
+  double wide;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (partials > 0) {
+  if (direct) {
     double norm;
-    norm_of(partial, partials, max_norm, &norm, &factor);
-    if (blockIdx.x == 0 && threadIdx.x == 0) { result[0] = static_cast<float>(norm); result[1] = factor; }
+    norm_of(partial, partials, max_norm, &norm, &wide);
+    if (blockIdx.x == 0 && threadIdx.x == 0) store_result(norm, wide, result);
   } else {
-    factor = result[1];
+    wide = partial[partials];
   }
+  const float factor = static_cast<float>(wide);
   const bool clip = factor != 1.0f;
   if (!clip && list.in_place) return;
   const int chunks = list.first[list.count];
+  if (wide > 0.0 && wide < SMALLEST_FACTOR) {
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+      const Chunk k = locate(list, c);
+      for (int i = threadIdx.x; i < k.n; i += THREADS) k.out[i] = static_cast<float>(static_cast<double>(k.g[i]) * wide);
+    }
+    return;
+  }
   int c = chunks - 1 - static_cast<int>(blockIdx.x);
   Chunk next = c >= 0 ? locate(list, c) : Chunk{};
   for (; c >= 0; c -= gridDim.x) {
@@ -226,7 +244,7 @@ int clip_all(cudaStream_t st, const int64_t* src, const int64_t* dst, const int6
     from = fill_list(&list, src, dst, sizes, from, count);
     if (list.count == 0) break;
     const int blocks = blocks_of(list.first[list.count], NORM_BLOCKS_PER_SM);
-    if (partials + blocks > work_doubles) return CU32_E_SCRATCH;
+    if (partials + blocks + 1 > work_doubles) return CU32_E_SCRATCH;
     grad_norm_kernel<CAP><<<blocks, THREADS, 0, st>>>(list, work + partials);
     if (cudaError_t e = cudaPeekAtLastError()) return static_cast<int>(e);
     partials += blocks;
@@ -235,7 +253,7 @@ int clip_all(cudaStream_t st, const int64_t* src, const int64_t* dst, const int6
   // One launch that every block of which can form the norm itself, or the norm first and a block per chunk behind it.
   const bool direct = scale && lists == 1 && list.first[list.count] <= device_sm_count() * CLIP_BLOCKS_PER_SM;
   if (!direct)
-    if (cudaError_t e = launch_behind(grad_result_kernel, 1, st, static_cast<const double*>(work), partials, max_norm, result))
+    if (cudaError_t e = launch_behind(grad_result_kernel, 1, st, work, partials, max_norm, result))
       return static_cast<int>(e);
   if (!scale || lists == 0) return CU32_OK;
   for (int from = 0; from < count;) {
@@ -245,7 +263,7 @@ int clip_all(cudaStream_t st, const int64_t* src, const int64_t* dst, const int6
     // in place the blocks may have nothing to do: fewer of them (12,000 that leave at once take 6 us)
     const int blocks = list.in_place ? blocks_of(list.first[list.count], 4 * CLIP_BLOCKS_PER_SM) : list.first[list.count];
     const cudaError_t e = launch_behind(grad_clip_kernel<CAP>, blocks, st, list,
-                                        static_cast<const double*>(work), direct ? partials : 0, max_norm, result);
+                                        static_cast<const double*>(work), partials, direct ? 1 : 0, max_norm, result);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   return CU32_OK;
@@ -278,7 +296,7 @@ using namespace dragon;
 extern "C" {
 
 long long cu32_gradClip_work(int count) {
-  // a launch holds 1000 tensors and leaves at most NORM_BLOCKS_PER_SM partial sums per SM
+  // a launch holds 1000 tensors and leaves at most NORM_BLOCKS_PER_SM partial sums per SM; one more for the factor
   if (count <= 0) return 0;
   return static_cast<long long>((count + 999) / 1000 + 1) * device_sm_count() * NORM_BLOCKS_PER_SM;
 }

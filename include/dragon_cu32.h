@@ -501,8 +501,10 @@ CU32_API int cu32_normResidual_delta(int64_t stream, const float* d_deltaRout, c
  *   overlap: in clipping a tensor is listed once), sizes: host array of their float counts (0 allowed).  The arrays are
  *   read during the call only.
  *   result: two device floats, {norm, factor}.  A tensor that stays in place is not touched where the factor is 1.
- *   A norm that is not finite (an infinity or NaN among the gradients) gives factor 1: nothing is scaled, and the caller
- *   sees the norm.  max_norm >= 0 (infinity allowed).
+ *   An infinity or NaN among the gradients gives a norm that is not finite and factor 1: nothing is scaled, and the caller
+ *   sees the norm.  Finite gradients are scaled by the 64-bit factor also where the two floats cannot hold it or the norm: a
+ *   norm above FP32's range is stored as infinity (beside a factor below 1), a factor below 2^-126 as FP32 rounds it.
+ *   max_norm >= 0 (infinity allowed).
  *   work: cu32_gradClip_work(count) device doubles of scratch; calls that may overlap need scratch of their own.
  * The norm does not vary from run to run.  cu32_gradNorm computes the norm alone (factor 1). */
 CU32_API long long cu32_gradClip_work(int count);

@@ -178,3 +178,26 @@ def test_clip_in_a_graph_and_beside_another(pkg, cuda):
         torch.cuda.synchronize()
         check(torch, results[0].tolist(), before, sets[0], 1.0)
     del graph
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2e36, 3e38], ids=str)
+@pytest.mark.parametrize("max_norm", [1.0, 1e-12, 1e30])
+@pytest.mark.parametrize("sizes", [[4099, 12, 7], [8000003], [3] * 1500], ids=lambda s: f"{len(s)}x{sum(s)}")
+def test_norms_and_factors_beyond_the_range_of_fp32(pkg, cuda, size, max_norm, sizes):
+    """Finite gradients whose norm, or whose factor, FP32 cannot hold: scaled as the formula says, one rounding off (two
+    where the factor is an FP32 number); the norm comes out as FP32 rounds it, infinite beyond its range."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(len(sizes))
+    grads = [size * (2 * torch.rand(n, device="cuda", generator=g) - 1) for n in sizes]
+    norm = norm64(grads)
+    factor = torch.tensor(max_norm, dtype=torch.float32).double().item() / norm      # the limit is an FP32 argument
+    for outs in ([torch.full_like(t, 7.0) for t in grads], [t.clone() for t in grads]):
+        in_place = torch.equal(outs[0], grads[0])
+        src = outs if in_place else grads
+        got_norm, got_factor = run(pkg, torch, src, outs, max_norm)
+        assert got_norm == math.inf if norm > 3.4028236e38 else abs(got_norm - norm) <= 1.01 * EPS * norm
+        assert abs(got_factor - factor) <= 1.01 * EPS * factor + 1e-45 and got_factor < 1.0
+        for a, o in zip(grads, outs):
+            want = a.double() * factor
+            assert ((o.double() - want).abs() <= 2.1 * EPS * want.abs() + 1e-45).all()
