@@ -15,6 +15,7 @@
 //   registers that hold the sums, and with the two products of deltaX in one accumulation.  6 N D F flop forward and
 //   12 N D F backward at the FP32-accurate rate bound it.
 #include <atomic>
+#include <initializer_list>
 
 #include "cu32_host.h"
 #include "gated_thin.h"
@@ -740,8 +741,10 @@ long long cu32_gatedFF_work(int N, int D, int F) {
   const long long b = extra(split_of(DUAL_TILES, 4, n, d, 2 * ((F + 31) / 32), any), n * d);  // deltaX
   const long long c = extra(split_of(PLAIN_TILES, 6, d, f, (N + 31) / 32, any), d * f);       // deltaWg, deltaWu
   const long long e = extra(split_of(PLAIN_TILES, 6, f, d, (N + 31) / 32, any), d * f);       // deltaWd
-  const long long m = a > b ? a : b, o = c > e ? c : e;
-  long long most = m > o ? m : o;
+  const long long h = extra(split_of(PLAIN_TILES, 6, n, f, (D + 31) / 32, any), n * f);       // deltaH
+  long long most = a;
+  for (const long long x : {b, c, e, h})
+    if (x > most) most = x;
   if (N > THIN_MAX_ROWS) return most;
   const long long forward = N > ROWS_MAX ? thin_floats(N, D, F) : 0, backward = thin_delta_floats(N, D, F);
   if (forward > most) most = forward;

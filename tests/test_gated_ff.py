@@ -555,3 +555,23 @@ def test_rows_give_up_key(pkg):
     v = ctypes.c_int(-5)
     assert lib.cu32_get_tune(b"rows_give_up", ctypes.byref(v)) == 0 and v.value == 0
     assert lib.cu32_tune(b"rows_give_up", 17) == -8 and lib.cu32_tune(b"rows_give_up", -1) == -8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(130, 8228, 68), (200, 20004, 36)], ids=str)
+def test_scratch_of_a_long_model_axis(pkg, cuda, shape):
+    """deltaH is a product over D: where D is long and F small it alone is cut through the scratch, whose size has to count
+    it."""
+    import gpu_util as G
+    torch = cuda
+    b = Block(torch, *shape, seed=80)
+    need = pkg.cu32.Cuda_gatedFF.work(*shape)
+    assert need >= shape[0] * shape[2]
+    work = torch.full((need + 64,), float("nan"), device="cuda")
+    b.forward(pkg, 0, work=work[:need])
+    check_forward(torch, b, 0)
+    work.fill_(float("nan"))
+    b.backward(pkg, 0, work=work[:need])
+    check_backward(torch, b, 0, b.get(torch, "G"), b.get(torch, "U"))
+    assert torch.isfinite(work[:shape[0] * shape[2]]).all() and torch.isnan(work[need:]).all()
+    G.check_status(pkg)
