@@ -644,9 +644,17 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
 // How a row of M floats is laid on a persistent kernel: blocks per row, vectors per block, working threads, and a ring of
 // rows of `arrays` parts that leaves room for the blocks an SM takes.
 constexpr int FORWARD_REGS = 64, DELTA_REGS = 96;      // what the kernels are compiled to at their launch bounds
+constexpr int FORWARD_SMEM = 640, DELTA_SMEM = 1664;   // their shared memory beside the ring
+// What an SM has: registers for a warp's 32 threads in each of its four parts, and shared memory, of which every block costs
+// 1 KB more than it asks for.
+constexpr int SM_PART_REGS = 16384, SM_SMEM = 228 * 1024, BLOCK_SMEM = 1024, SM_BLOCKS = 32;
+constexpr int MOST_RING = 220 * 1024;                  // dynamic shared memory of a block
+// A plan takes 220 KB and 2 KB per block beside the rings: what is left of the 228 KB is the L1 cache's (8192 x 1136, both
+// calls: 80 us; filled to the brim 89).
+constexpr int PLAN_SMEM = 220 * 1024, PLAN_BLOCK = 2048;
 struct Shape { int cl, vecs, threads, stages, stage_bytes, slab_bytes, per_sm; };
 
-Shape ring_shape(int M, int arrays, int regs) {
+Shape ring_shape(int M, int arrays, int regs, int smem) {
   Shape s{};
   const int all = M / 4;
   s.cl = all <= 1024 ? 1 : (all <= 2048 ? 2 : 4);
@@ -657,11 +665,16 @@ Shape ring_shape(int M, int arrays, int regs) {
   // Blocks per SM: by shared memory and by the registers per thread.  Three rows in a ring, but two in a cluster's, whose
   // exchange of sums a second block covers better than a third row (gradients of 8192 x 5000: 161 us, with three 213;
   // single blocks of 256 columns: 52 us with three, 63 with two).
-  const int rows = s.cl == 1 ? 3 : 2, by_smem = 220 * 1024 / (rows * s.stage_bytes + 2048), by_regs = 65536 / (regs * s.threads);
-  s.per_sm = by_smem < by_regs ? by_smem : by_regs;
+  // No more than are resident at a time: a block left over would start when one of the others has done all its rows (gradients
+  // of 8192 x 620, 6 blocks to an SM, with the forward: 55 us, planned with 7: 62).
+  auto least = [](int a, int b) { return a < b ? a : b; };
+  const int ring = (s.cl == 1 ? 3 : 2) * s.stage_bytes, fixed = smem + BLOCK_SMEM;
+  const int by_smem = least(PLAN_SMEM / (ring + PLAN_BLOCK), SM_SMEM / (ring + fixed));
+  const int by_regs = 4 * (SM_PART_REGS / (regs * 32)) / (s.threads / 32);
+  s.per_sm = least(least(by_smem, by_regs), SM_BLOCKS);
   if (s.per_sm < 1) s.per_sm = 1;
-  s.stages = (220 * 1024 / s.per_sm - 2048) / s.stage_bytes;
-  if (s.stages > MAX_STAGES) s.stages = MAX_STAGES;
+  s.stages = least(PLAN_SMEM / s.per_sm - PLAN_BLOCK, SM_SMEM / s.per_sm - fixed) / s.stage_bytes;
+  s.stages = least(s.stages, MAX_STAGES);
   return s;
 }
 
@@ -684,7 +697,7 @@ int cluster_count() {
   attr[0].val.clusterDim.z = 1;
   q.attrs = attr;
   q.numAttrs = 1;
-  if (cudaFuncSetAttribute(norm_delta_kernel<CL, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) !=
+  if (cudaFuncSetAttribute(norm_delta_kernel<CL, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_RING) !=
           cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&n, norm_delta_kernel<CL, true, true>, &q) != cudaSuccess || n < 1) {
     cudaGetLastError();      // no device, or none that could run it: the launch will say so
@@ -707,7 +720,7 @@ cudaError_t launch_ring(const Shape& s, NormParams p, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (!ready[dev & 63].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_RING);
     if (e != cudaSuccess) return e;
     ready[dev & 63].store(1, std::memory_order_release);
   }
@@ -804,7 +817,7 @@ int cu32_normResidual(int64_t stream, const float* B, const float* R, const floa
     else norm_forward_kernel<4><<<N, threads, 0, st>>>(p);
     return static_cast<int>(cudaPeekAtLastError());
   }
-  const Shape s = ring_shape(M, 2, FORWARD_REGS);
+  const Shape s = ring_shape(M, 2, FORWARD_REGS, FORWARD_SMEM);
   p.units = ring_units(s);
   if (p.units > N) p.units = N;
   if (s.cl == 1) return static_cast<int>(launch_ring<norm_forward_ring_kernel<1>>(s, p, st));
@@ -814,7 +827,7 @@ int cu32_normResidual(int64_t stream, const float* B, const float* R, const floa
 
 long long cu32_normResidual_work(int N, int M, int gate_rows) {
   if (check_rows(N, M, M, gate_rows)) return 0;
-  return work_floats_of(plan_rows(N, gate_rows, ring_units(ring_shape(M, 4, DELTA_REGS))), M);
+  return work_floats_of(plan_rows(N, gate_rows, ring_units(ring_shape(M, 4, DELTA_REGS, DELTA_SMEM))), M);
 }
 
 int cu32_normResidual_delta(int64_t stream, const float* dRout, const float* dY, const float* B, const float* Rout,
@@ -826,7 +839,7 @@ int cu32_normResidual_delta(int64_t stream, const float* dRout, const float* dY,
   if (int rc = check_rows(N, M, width, gate_rows)) return rc;
   if (gate && gate_rows == 0) return CU32_E_DIM;
   if (!all_aligned16(dRout, dY, B, Rout, gate, wpost, wpre, dR, dB, dgate, dwpost, dwpre, work)) return CU32_E_ALIGN;
-  const Shape s = ring_shape(M, 4, DELTA_REGS);
+  const Shape s = ring_shape(M, 4, DELTA_REGS, DELTA_SMEM);
   int want = ring_units(s);
   const long long room = work_floats / (3LL * M);
   if (room < 1) return CU32_E_SCRATCH;

@@ -162,6 +162,19 @@ def test_norm_residual_refusals(pkg):
         pkg.cu32.Cuda_normResidual.normResidual(0, P, P, 0, 0, P, P, P, P, 0, 0, 0, 8, 8, 1.0, 1.0, 1e-6)
 
 
+def test_norm_blocks_are_resident(pkg):
+    """The gradients' scratch has a row per block; there are no more of them than an SM holds at a time: 96 registers a thread,
+    so 5 warps in each of its four parts, and 228 KB of shared memory for rings of three rows, 1664 bytes and 1 KB a block."""
+    import torch
+    sms = torch.cuda.get_device_properties(0).multi_processor_count if torch.cuda.is_available() else 1
+    for M in range(4, 4097, 4):
+        units = pkg.cu32.Cuda_normResidual.work(1 << 28, M, 0) // (3 * M)
+        warps = ((M // 4 + 1) // 2 + 31) // 32
+        ring = 3 * ((M * 16 + 127) // 128 * 128)
+        fits = min(20 // warps, 228 * 1024 // (ring + 1664 + 1024))
+        assert 1 <= units / sms <= fits, M
+
+
 # ---------------------------------------------------------------------------------------------------- on the GPU
 WIDTHS = [1, 3, 4, 31, 127, 128, 129, 513, 1000, 1024, 2051, 4096, 4099, 8192, 8195, 16381, 16384]
 
