@@ -36,6 +36,7 @@ static std::atomic<int> g_ring_paired{1};
 static std::atomic<int> g_ring_fixed{1};
 static std::atomic<int> g_phase_fused{1};
 static std::atomic<int> g_rows_give_up{0};
+static std::atomic<int> g_column_cuts{0};
 
 void load_env_once() {
   static std::once_flag once;
@@ -168,6 +169,7 @@ static int pick_tile(long long M, int N, long long z) {
 // Also sets how many chunks are summed in registers between flushes to memory: 256 k-blocks (K = 8192).
 int forced_tile() { return g_tile.load(); }
 int rows_give_up() { return g_rows_give_up.load(); }
+void note_column_cut() { ++g_column_cuts; }
 void choose_rings(GemmParams* p) {
   p->flush_chunks = 256 / p->kc > 1 ? 256 / p->kc : 1;
   p->ring_raw = g_ring_raw.load();
@@ -1493,6 +1495,7 @@ int cu32_get_tune(const char* key, int* value) {
   if (!std::strcmp(key, "phase_fused")) { *value = g_phase_fused; return CU32_OK; }
   if (!std::strcmp(key, "rows_give_up")) { *value = g_rows_give_up; return CU32_OK; }
   if (!std::strcmp(key, "sm_reserve")) { *value = g_sm_reserve; return CU32_OK; }
+  if (!std::strcmp(key, "column_cuts")) { *value = g_column_cuts; return CU32_OK; }
   if (!std::strcmp(key, "last_tile")) { *value = g_last_tile; return CU32_OK; }
   return CU32_E_ARG;
 }

@@ -55,6 +55,8 @@ int make_map3_as(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, ui
 constexpr int GATED_KC = 1;
 // The "tile" tuning key: a forced tile configuration, or -1.
 int forced_tile();
+// Counts a product that went in two pieces of columns for the "column_cuts" tuning key.
+void note_column_cut();
 // The "rows_give_up" tuning key.
 int rows_give_up();
 // Ring lengths, flush interval, clock accumulator and reserved SMs of a launch, from the tuning integers.

@@ -572,6 +572,7 @@ int product(const int64_t* s, bool a_mn, bool b_mn, const float* A, long long ld
   c.N = c.n_store = plan.first_cols;
   if (int rc = run_gemm(c)) return rc;
   if (plan.first_cols == N) return CU32_OK;
+  note_column_cut();
   c.B = b_mn ? B + plan.first_cols : B + plan.first_cols * ldb;
   c.C = C + plan.first_cols;
   c.N = c.n_store = N - plan.first_cols;
@@ -624,6 +625,7 @@ int gated_tiles(const float* X, const float* Wg, const float* Wu, float* G, floa
   const ColumnPlan c = plan_columns(GATED_TILES, 3, N, F, (D + 31) / 32, 2);
   if (int rc = gated_part(X, Wg, Wu, G, U, H, N, D, F, act, 0, c.first_cols, c.first_tile, false, st)) return rc;
   if (c.first_cols == F) return CU32_OK;
+  note_column_cut();
   return gated_part(X, Wg, Wu, G, U, H, N, D, F, act, c.first_cols, F - c.first_cols, c.rest_tile, true, st);
 }
 

@@ -544,6 +544,7 @@ CU32_API int cu32_gradClip(int64_t stream, const int64_t* src, const int64_t* ds
  *   "sm_reserve" SMs the contraction kernel's persistent grid leaves free, for kernels a host runs beside it on
  *              another stream (a collective that reassembles output shards); 0 = none (default)
  *   "last_tile" (read only) tile configuration of the most recent contraction call of this process
+ *   "column_cuts"     (read only) how many products of the gated block this process has run in two pieces of columns
  *   "rows_give_up"    (tests) in the gated block's forward call of up to 8 rows one warp of block 0 counts a wait as run out:
  *              1..8 = warp 0..7 its first wait for a weight tile, 9..16 its first wait for a column block's sums; the kernel
  *              returns with the status word set, its results are incomplete; 0 = none (default)

@@ -575,3 +575,48 @@ def test_scratch_of_a_long_model_axis(pkg, cuda, shape):
     check_backward(torch, b, 0, b.get(torch, "G"), b.get(torch, "U"))
     assert torch.isfinite(work[:shape[0] * shape[2]]).all() and torch.isnan(work[need:]).all()
     G.check_status(pkg)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,scratch,cut", [
+    # the gated launch; it and deltaH; deltaWd, deltaWg and deltaWu, deltaH beside a deltaWd in two pieces; Y
+    ((400, 260, 5124), True, (1, 0)), ((1000, 260, 5124), True, (1, 1)), ((260, 1028, 4100), True, (0, 3)),
+    ((260, 1028, 4100), False, (0, 3)), ((1021, 2048, 5464), True, (1, 2)), ((1021, 2048, 5464), False, (1, 3)),
+    ((2048, 2048, 5464), True, (0, 3)), ((1000, 5124, 1028), False, (1, 3)), ((1300, 3588, 516), True, (1, 0)),
+], ids=str)
+def test_products_in_two_pieces_of_columns(pkg, cuda, shape, scratch, cut):
+    """Columns that fill whole rounds of tiles, and the rest in smaller tiles beside the last round: the offsets of the second
+    piece, and what stands beside or behind it.  The counter says that the cuts were made."""
+    import gpu_util as G
+    torch = cuda
+
+    def cuts():
+        v = ctypes.c_int()
+        assert pkg.cu32.load().cu32_get_tune(b"column_cuts", ctypes.byref(v)) == 0
+        return v.value
+    b = Block(torch, *shape, seed=81)
+    n = pkg.cu32.Cuda_gatedFF.work(*shape) if scratch else 0
+    work = torch.full((n,), float("nan"), device="cuda") if n else None
+    counts = [cuts()]
+    b.forward(pkg, 0, work=work)
+    counts.append(cuts())
+    b.backward(pkg, 0, work=work)
+    counts.append(cuts())
+    assert (counts[1] - counts[0], counts[2] - counts[1]) == cut
+    check_forward(torch, b, 0)
+    check_backward(torch, b, 0, b.get(torch, "G"), b.get(torch, "U"))
+    names = ("dX", "dWg", "dWu", "dWd")
+    want = {n: b.get(torch, n) for n in ("dG", "dU", "Y") + names}
+    kept = {n: getattr(b, n).view.clone() for n in "GUH"}
+    for over in (None, "U", "G"):                 # the same bits again, and with deltaG over H, deltaU over U or G
+        for n in names:
+            getattr(b, n).view.fill_(float("nan"))
+        b.backward(pkg, 0, work=work, over=over)
+        assert torch.equal(b.get(torch, "H" if over else "dG"), want["dG"]) and torch.equal(b.get(torch, over or "dU"), want["dU"])
+        for n in names:
+            assert torch.equal(b.get(torch, n), want[n]), (over, n)
+        for n in "GUH":
+            getattr(b, n).view.copy_(kept[n])
+    b.forward(pkg, 0, save=False, work=work)
+    assert torch.equal(b.get(torch, "Y"), want["Y"])
+    G.check_status(pkg)
