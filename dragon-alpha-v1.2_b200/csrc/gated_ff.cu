@@ -431,7 +431,7 @@ int rows_shape(const RowsCall& c, cudaStream_t st) {
   double best = 1e300;
   for (int w = 128; w >= 32; w >>= 1)
     for (int s = 1; s <= 4; s <<= 1) {
-      const int ktiles = (c.K * w + 4095) / 4096;
+      const int ktiles = static_cast<int>((static_cast<long long>(c.K) * w + 4095) / 4096);
       if (ktiles < s) continue;
       const int items = (c.M + w - 1) / w, clusters = s == 4 ? sms * 2 / 9 : sms / s;
       const double rounds = (items + clusters - 1) / clusters;
