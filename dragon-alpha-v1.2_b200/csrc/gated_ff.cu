@@ -6,11 +6,12 @@
 //
 // Three forms, by what bounds them:
 // Up to 8 rows, forward: every weight is read once for all rows by FP32 multiply-adds, so the time is that of reading
-//   3 D F floats (rows_kernel below; 4096 / 10924, 537 MB: 93 us for one row, 103 us for 8).  The multiply-adds fill the
-//   issue slots beyond: 16 rows would take as long as two calls.
+//   3 D F floats (rows_kernel below; 4096 / 10924, 537 MB: 92 us for one row, 102 us for 8, in a long graph; a call by
+//   itself 109 to 113 us for 8).  The multiply-adds fill the issue slots beyond: 16 rows would take as long as two calls.
 // Up to 128 rows: the same reading bounds it, but the products run on the tensor cores with the weights as the tile's
-//   rows (gemm_thin.cu; 16 rows 117 us, 128 rows 251 us, where the tiles below take 315 and 320 us); it needs scratch.
-//   The gradients use it from one row on, with all weight gradients in one launch up to 24 rows (gated_outer.cu).
+//   rows (gemm_thin.cu; 16 rows 119 us, 128 rows 264 us, where the tiles below took 315 and 320 us with a cut second
+//   product); it needs scratch, without it these calls take 490 to 500 us.  The gradients use it from one row on, with all
+//   weight gradients in one launch up to 24 rows (gated_outer.cu).
 // More rows: the contraction kernel (gemm_tf32.cuh) with both projections in one launch and act(G) * U formed in the
 //   registers that hold the sums, and with the two products of deltaX in one accumulation.  6 N D F flop forward and
 //   12 N D F backward at the FP32-accurate rate bound it.
@@ -102,8 +103,8 @@ struct RowsCfg {
 // columns, with the KT columns of X that meet them) full by TMA whatever the workers do; the persistent cluster takes
 // blocks of CPW columns in turn, its S blocks a slice of K each.  A worker holds 4 columns x NR rows of sums; the sums of
 // lanes, warps and blocks are added in a fixed order, each block of the cluster finishing CPW / S columns.
-// (Measured for 8 rows of a 4096 / 10924 block, 537 MB: 103 us, 5.2 TB/s; with plain loads into registers instead of the
-// ring, one launch over all column blocks, 184 us.)
+// (Measured for 8 rows of a 4096 / 10924 block, 537 MB: 102 us in a long graph, 5.2 TB/s, and 109 us, 4.9 TB/s, for calls one
+// by one; with plain loads into registers instead of the ring, one launch over all column blocks, 184 us.)
 template <int NR, int MATS, int CPW, int S>
 __global__ void __launch_bounds__(ROWS_THREADS, 1) rows_kernel(const __grid_constant__ RowsParams p) {
   using Cfg = RowsCfg<NR, MATS, CPW, S>;
@@ -615,7 +616,9 @@ int gated_part(const float* X, const float* Wg, const float* Wu, float* G, float
   if (int rc = fill_common(&p, N, cols, nkb, tile, tile_bn(tile) / 2)) return rc;
   p.C = H + c0; p.ldc = F; p.act = act; p.tma_store = 1;
   p.overlap_prev = p.join_prev = beside ? 1 : 0;
-  p.flush_chunks = nkb;      // one flush: the activation needs the complete sums
+  // One flush: the activation needs the complete sums.  Beyond D = 8192, where plain products put their registers' sums down
+  // in memory, these chains of D / 32 additions go on: 3.6e-7 off at D = 8192, 4.7e-7 at 16384, 8.3e-7 at 65536.
+  p.flush_chunks = nkb;
   return static_cast<int>(launch_gemm_gated(tile, p, st));
 }
 

@@ -17,8 +17,8 @@
 // rows.  (Equal runs of a list ordered column block by column block balance better, but read scattered 512-byte pieces:
 // 4 TB/s, and asking for them earlier made it slower still.)  A slice's sums go to the caller's scratch and a second kernel
 // adds a column block's slices in order, applies the gate and stores the rows (no atomics: results do not vary).
-// Measured for a 4096 / 10924 block, forward: 16 rows 117 us (the reads at 4.8 TB/s), 32 rows 140, 64 rows 160, 128 rows
-// 251 us, where X and its parts weigh as much as the weights.
+// Measured for a 4096 / 10924 block, forward, in a long graph: 16 rows 119 to 122 us (the reads at 4.8 TB/s), 32 rows 139 to
+// 143, 64 rows 168 to 173, 128 rows 264 to 276 us, where X and its parts weigh as much as the weights.
 #include <atomic>
 
 #include "cu32_host.h"

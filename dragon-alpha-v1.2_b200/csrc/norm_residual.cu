@@ -35,8 +35,9 @@ constexpr int MAX_WIDTH = 16384;     // floats per row: a cluster of four blocks
 // every row made the kernels wait for it (with four per thread: 145 us forward, 213 us gradients at 8192 x 4096).
 constexpr int VPT = 2;
 constexpr int RING_THREADS = 512;
-// Holds the gradient kernel to 96 registers, without spills (a block has at most RING_THREADS threads; left to itself it takes
-// 118, and one block of 288 threads fills an SM instead of two: 8192 x 2052 rows 89 us instead of 79; elsewhere the same).
+// Holds the gradient kernel to 96 registers (a block has at most RING_THREADS threads; left to itself it takes 118, and one
+// block of 288 threads fills an SM instead of two: 8192 x 2052 rows 89 us instead of 79; elsewhere the same).  Of its twelve
+// instances one spills, the clusters of two with gate and both norms: 8 bytes stored, 4 read again.
 constexpr int DELTA_BOUND = 576;
 
 __device__ __forceinline__ float4 ldg_row(const float* p) {       // read once: not kept in L1
